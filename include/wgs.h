@@ -570,6 +570,36 @@ int wgs_attn_fwd(const float* theta, const float* phi, const float* g, float* o,
 int wgs_attn_bwd(const float* theta, const float* phi, const float* g, const float* o, const float* lse, const float* d_o, float* ws,
                  float* dtheta, float* dphi, float* dg, int B, int Pq, int Pk, int c8, int c2, wgs_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Element types of the entry points below that take `const void*` with a dtype.
+ */
+#define WGS_F32 0
+#define WGS_BF16 1
+#define WGS_F16 2
+
+/* ------------------------------------------------------------------------------------------------
+ * Log-probabilities of given labels, with the entropy of the scores and the `top` most likely alternatives, and their gradient — the
+ * classification term of the step (lib/trainer.py:245-258) as an operator of its own: any label count, row stride and type, differentiable
+ * in every output.  Per row of V scores l:
+ *     p = softmax(l),   logp = log p_label,   entropy = -sum p log p,   (top_logp, top_index)[j] = the j-th largest log p (ties: lower index)
+ *   logits    [rows, V] of dtype, row_stride elements apart, aligned to the type only
+ *   labels    [rows] int64; ignore_index: logp 0, no gradient of its own (entropy and alternatives are computed as ever); any other value
+ *             outside [0, V): logp and the row's gradient NaN
+ *   logp, entropy [rows], top_logp / top_index [rows, top] (NULL when top = 0): fp32 / int64
+ *   stat      [rows, 2] fp32 (max, log of the sum): read by the backward
+ *   ws        wgs_label_logprobs_ws_bytes() bytes, 16-byte aligned (0: may be NULL); written and read within the call
+ * A row of nothing but minus infinity has logp and top_logp minus infinity, entropy 0 and gradient 0; one with a NaN or plus infinity has NaN
+ * throughout and top_index -1.  rows < 2^24, V < 2^30, top <= 64.
+ * Backward: g_logp / g_entropy [rows], g_top [rows, top] (any may be NULL) -> grad [rows, V] of dtype, grad_row_stride apart, every element of
+ * [0, V) of a row overwritten; grad may not overlap logits.
+ */
+int64_t wgs_label_logprobs_ws_bytes(int64_t rows, int64_t V, int top);
+int wgs_label_logprobs_fwd(const void* logits, int dtype, int64_t rows, int64_t V, int64_t row_stride, const int64_t* labels, int64_t ignore_index, int top,
+                           float* logp, float* entropy, float* stat, float* top_logp, int64_t* top_index, void* ws, int64_t ws_bytes, wgs_stream_t stream);
+int wgs_label_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t V, int64_t row_stride, const int64_t* labels, int64_t ignore_index,
+                           const float* stat, const float* entropy, int top, const int64_t* top_index, const float* g_logp, const float* g_entropy,
+                           const float* g_top, void* grad, int64_t grad_row_stride, wgs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,7 +1,13 @@
 """Operator-level mirror of the reference's native seam `models/StyleGAN2/op` (op/__init__.py:1-2):
 `FusedLeakyReLU`, `fused_leaky_relu`, `upfirdn2d` — same names, arguments and autograd behaviour,
 backed by the C ABI (wgs_bias_act / wgs_upfirdn2d) instead of the JIT-built CUDA extension.
+
+Beside it, the operators that close a training step: `label_logprobs` (log-probabilities of given labels, entropy, top alternatives, and
+their gradient).
 """
+import collections
+import contextlib
+
 import torch
 from torch import nn
 
@@ -105,3 +111,99 @@ class _UpFirDn2d(torch.autograd.Function):
 
 def upfirdn2d(x, kernel, up=1, down=1, pad=(0, 0)):
     return _UpFirDn2d.apply(x, kernel, (up, up), (down, down), (pad[0], pad[1], pad[0], pad[1]))
+
+
+# ---- operators of the training objective -------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # WGS_F32 / WGS_BF16 / WGS_F16
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Context in which launches go to `device`'s current stream, whatever the current device is."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+LabelLogprobs = collections.namedtuple('LabelLogprobs', 'logp entropy top_logp top_index')
+TOP_MAX = 64
+
+
+def _rows_of(x):
+    """(x viewed or copied as [rows, V] with adjacent scores and rows that do not overlap, row stride in elements)."""
+    V = x.shape[-1]
+    if x.dim() != 2:
+        x = x.reshape(-1, V)
+    if (V > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    return x, (x.stride(0) if x.shape[0] > 1 else V)
+
+
+class _LabelLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, top, ignore_index):
+        dev, V = logits.device, logits.shape[-1]
+        x, stride = _rows_of(logits)
+        rows = x.shape[0]
+        code = _DTYPES[x.dtype]
+        lead = logits.shape[:-1]
+        with _on(dev):
+            logp = torch.empty(lead, device=dev)
+            entropy = torch.empty(lead, device=dev)
+            stat = torch.empty(rows, 2, device=dev)
+            top_logp = torch.empty(lead + (top,), device=dev)
+            top_index = torch.empty(lead + (top,), dtype=torch.int64, device=dev)
+            need = L.lib().wgs_label_logprobs_ws_bytes(L.c_int64(rows), L.c_int64(V), top)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            L.check(L.lib().wgs_label_logprobs_fwd(L.rawptr(x), code, L.c_int64(rows), L.c_int64(V), L.c_int64(stride), L.rawptr(labels),
+                                                   L.c_int64(ignore_index), top, L.rawptr(logp), L.rawptr(entropy), L.rawptr(stat),
+                                                   L.rawptr(top_logp), L.rawptr(top_index), L.rawptr(ws), L.c_int64(need), L.stream()),
+                    'wgs_label_logprobs_fwd')
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(top_index)
+        # (a copy made of a strided input is saved in its place)
+        ctx.save_for_backward(x if x.data_ptr() != logits.data_ptr() else logits, labels, stat, entropy, top_index)
+        ctx.cfg = (top, ignore_index, logits.shape)
+        return logp, entropy, top_logp, top_index
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, labels, stat, entropy, top_index = ctx.saved_tensors
+        top, ignore_index, shape = ctx.cfg
+        dev, V = logits.device, shape[-1]
+        x, stride = _rows_of(logits)
+        rows, size = x.shape[0], x.element_size()
+        with _on(dev):
+            up = [None if g is None else g.to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_top)]
+            # rows of the gradient start at the same place of a 16-byte block as those of the logits: whole-vector reads and writes
+            per = 16 // size
+            first = x.data_ptr() % 16 // size
+            gstride = V + (stride - V) % per if rows > 1 else V
+            buf = torch.empty(first + rows * gstride, dtype=x.dtype, device=dev)
+            grad = buf[first:].view(rows, gstride)[:, :V]
+            L.check(L.lib().wgs_label_logprobs_bwd(L.rawptr(x), _DTYPES[x.dtype], L.c_int64(rows), L.c_int64(V), L.c_int64(stride),
+                                                   L.rawptr(labels), L.c_int64(ignore_index), L.rawptr(stat), L.rawptr(entropy), top,
+                                                   L.rawptr(top_index), L.rawptr(up[0]), L.rawptr(up[1]), L.rawptr(up[2]),
+                                                   L.rawptr(grad), L.c_int64(gstride), L.stream()), 'wgs_label_logprobs_bwd')
+        return grad.view(shape) if len(shape) != 2 and gstride == V else grad.reshape(shape), None, None, None
+
+
+def label_logprobs(logits, labels, top=0, ignore_index=-100):
+    """Log-probability of each row's label under softmax(logits), the entropy of the row, and its `top` most likely classes.
+
+    logits [..., V] (float32 / bfloat16 / float16, any strides; rows with adjacent scores are read in place), labels [...] int64.
+    -> LabelLogprobs(logp [...], entropy [...], top_logp [..., top], top_index [..., top]): float32, int64 indices, equal scores in the order
+    of their indices.  A label equal to ignore_index has logp 0 and passes no gradient; one that is no class otherwise gives NaN.  Rows of
+    nothing but -inf: logp -inf, entropy 0, gradient 0; rows with a NaN or +inf: NaN, top_index -1.  top <= 64.
+    Differentiable in logp, entropy and top_logp (the loss and the statistics of lib/trainer.py:245-258 are made of them)."""
+    if not logits.is_cuda:
+        raise L.WgsError("logits must be a GPU tensor (the HIP path has no CPU fallback)")
+    if logits.dtype not in _DTYPES:
+        raise L.WgsError("logits must be float32, bfloat16 or float16, got %s" % logits.dtype)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise L.WgsError("logits must have at least one class, got shape %s" % (tuple(logits.shape),))
+    if labels.dtype != torch.int64 or labels.device != logits.device or labels.shape != logits.shape[:-1]:
+        raise L.WgsError("labels must be int64 of shape %s on %s, got %s %s on %s" % (
+            tuple(logits.shape[:-1]), logits.device, labels.dtype, tuple(labels.shape), labels.device))
+    if not 0 <= top <= min(TOP_MAX, logits.shape[-1]):
+        raise L.WgsError("top must be 0 .. %d (and at most the number of classes), got %d" % (TOP_MAX, top))
+    return LabelLogprobs(*_LabelLogprobsFn.apply(logits, labels.contiguous(), int(top), int(ignore_index)))
