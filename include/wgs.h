@@ -600,6 +600,36 @@ int wgs_label_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t 
                            const float* stat, const float* entropy, int top, const int64_t* top_index, const float* g_logp, const float* g_entropy,
                            const float* g_top, void* grad, int64_t grad_row_stride, wgs_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Orthogonalised updates (in place of torch.optim.Adam's, lib/trainer.py:153-156, for the weights that are matrices).
+ * wgs_orthogonalise: out = X_steps of  X_0 = in / (|in|_F + eps),  X_{t+1} = (a + b A_t + c A_t^2) X_t,  A_t = X_t X_t^T  (the transposed
+ * iteration where rows > cols): with (a, b, c) = (3.4445, -4.7750, 2.0315) and 5 steps the singular values of `in` go to about 1, its
+ * singular vectors stay.  A zero matrix gives zeros; one with a NaN or infinity gives NaN throughout.
+ * wgs_muon_step, per matrix: momentum <- mu momentum + grad_scale in;  u = grad_scale in + mu momentum (nesterov) or momentum;
+ *     out <- decay out - step * (X_steps of u)       (in = gradient, out = weight; decay = 1 - lr weight_decay, step = lr * the shape's factor)
+ * Any number of matrices of any sizes goes through the same few launches.  in / out of dtype, rows `row_stride` apart (elements within a row
+ * adjacent), `batch` instances `batch_stride` apart (in: 0 repeats one); momentum fp32 [batch, rows, cols] contiguous (wgs_muon_step only).
+ * The matrices of a call may not overlap where they are written; in == out is allowed.  rows * cols (padded to 32) < 2^30.
+ * steps 1 .. 16; coefficients whose iterates leave 1e6 are refused.  Differentiable it is not.
+ * ws: *_ws_bytes() of the same matrices (pointers may be NULL in that call's batch = 0 entries only), 256-byte aligned; contents do not matter
+ * before or after the call.
+ */
+typedef struct wgs_matrix {
+    const void* in;
+    void* out;
+    float* momentum;
+    int64_t in_batch_stride, out_batch_stride, in_row_stride, out_row_stride;
+    int rows, cols, batch;
+    float step, decay;
+    int reserved;
+} wgs_matrix;
+int64_t wgs_orthogonalise_ws_bytes(const wgs_matrix* mats, int count, int dtype, int steps);
+int wgs_orthogonalise(const wgs_matrix* mats, int count, int dtype, int steps, float a, float b, float c, float eps, void* ws, int64_t ws_bytes,
+                      wgs_stream_t stream);
+int64_t wgs_muon_step_ws_bytes(const wgs_matrix* mats, int count, int dtype, int steps);
+int wgs_muon_step(const wgs_matrix* mats, int count, int dtype, float momentum, int nesterov, float grad_scale, int steps, float a, float b, float c,
+                  float eps, void* ws, int64_t ws_bytes, wgs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

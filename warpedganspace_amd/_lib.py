@@ -61,7 +61,7 @@ def lib():
         _lib.wgs_rbf_ws_floats.restype = ctypes.c_int64
         _lib.wgs_dev_launch_count.restype = ctypes.c_int64
         _lib.wgs_dev_last_kernel.restype = ctypes.c_char_p
-        for name in ("wgs_conv_ws_bytes", "wgs_label_logprobs_ws_bytes"):
+        for name in ("wgs_conv_ws_bytes", "wgs_label_logprobs_ws_bytes", "wgs_orthogonalise_ws_bytes", "wgs_muon_step_ws_bytes"):
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = ctypes.c_int64
     return _lib

@@ -3,10 +3,12 @@
 backed by the C ABI (wgs_bias_act / wgs_upfirdn2d) instead of the JIT-built CUDA extension.
 
 Beside it, the operators that close a training step: `label_logprobs` (log-probabilities of given labels, entropy, top alternatives, and
-their gradient).
+their gradient), `orthogonalise` (orthogonal factor of an update) and `muon_step` (momentum, orthogonalisation, weight update).
 """
 import collections
 import contextlib
+import ctypes
+import struct
 
 import torch
 from torch import nn
@@ -207,3 +209,157 @@ def label_logprobs(logits, labels, top=0, ignore_index=-100):
     if not 0 <= top <= min(TOP_MAX, logits.shape[-1]):
         raise L.WgsError("top must be 0 .. %d (and at most the number of classes), got %d" % (TOP_MAX, top))
     return LabelLogprobs(*_LabelLogprobsFn.apply(logits, labels.contiguous(), int(top), int(ignore_index)))
+
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # the quintic whose iterates take singular values of (0, 1] to about 1 in five steps
+_MATRIX = struct.Struct('=3Q4q3i2fi')            # wgs_matrix of include/wgs.h
+
+
+def _run_matrices(entries, ws_bytes, call, dtype, device, steps):
+    """entries: packed wgs_matrix fields of every matrix; call(mats, count, dtype code, workspace, its bytes)."""
+    n = len(entries)
+    mats = ctypes.create_string_buffer(_MATRIX.size * n)
+    for i, e in enumerate(entries):
+        _MATRIX.pack_into(mats, i * _MATRIX.size, *e)
+    code = _DTYPES[dtype]
+    with _on(device):
+        need = ws_bytes(mats, n, code, steps)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        call(mats, n, code, L.rawptr(ws), L.c_int64(need))
+
+
+def _as_rows(x):
+    """[batch, M, N] view (or copy) of x [..., M, N] with adjacent elements in a row."""
+    M, N = x.shape[-2:]
+    y = x if x.dim() == 3 else x.reshape(-1, M, N)
+    b, r, c = y.stride()
+    if (N > 1 and c != 1) or (M > 1 and r < N) or (y.shape[0] > 1 and b < 0):
+        y = y.contiguous()
+    return y
+
+
+def _strides(y):
+    """(batch stride, row stride) of a [batch, M, N] tensor, as the kernels want them where a dimension has one entry."""
+    _, M, N = y.shape
+    r = y.stride(1) if M > 1 else N
+    return (y.stride(0) if y.shape[0] > 1 else M * r), r
+
+
+def _check_matrix(x, what, device=None, dtype=None):
+    if not x.is_cuda:
+        raise L.WgsError("%s must be a GPU tensor (the HIP path has no CPU fallback)" % what)
+    if x.dtype not in _DTYPES:
+        raise L.WgsError("%s must be float32, bfloat16 or float16, got %s" % (what, x.dtype))
+    if x.dim() < 2 or x.shape[-1] < 1 or x.shape[-2] < 1:
+        raise L.WgsError("%s must be [..., M, N] with M, N >= 1, got shape %s" % (what, tuple(x.shape)))
+    if device is not None and (x.device != device or x.dtype != dtype):
+        raise L.WgsError("%s: the tensors of a call must share device and type, got %s on %s beside %s on %s" % (what, x.dtype, x.device, dtype, device))
+
+
+def orthogonalise(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
+    """Orthogonal factor of x [..., M, N] by the quintic Newton-Schulz iteration: X / (|X|_F + eps), then `steps` times
+    X <- (a + b A + c A A) X, A = X X^T (on the transposed matrix where M > N).  With the default coefficients singular values go to about 1
+    (0.7 .. 1.2) and singular vectors stay.
+
+    x: float32 / bfloat16 / float16, any strides; or a list of such matrices, of any sizes, which then share the launches.  Returns a new tensor
+    (list) of the same type.  The products keep fp32's precision whatever the type (fp16 hi + lo operands, fp32 sums).  A matrix of zeros
+    gives zeros, one with a NaN or infinity NaN throughout.  Not differentiable: an update rule's operator, for use without gradients."""
+    many = isinstance(x, (list, tuple))
+    xs = list(x) if many else [x]
+    if not xs:
+        return []
+    for t in xs:
+        _check_matrix(t, 'x', xs[0].device, xs[0].dtype)
+        if t.requires_grad and torch.is_grad_enabled():
+            raise L.WgsError("orthogonalise has no gradient: call it under torch.no_grad() or on a detached tensor")
+    entries, outs, keep = [], [], []
+    for t in xs:
+        swap = t.stride(-1) != 1 and t.stride(-2) == 1 and t.shape[-1] > 1       # columns adjacent: orthogonalise the transposed view
+        y = _as_rows(t.mT if swap else t)
+        out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        keep.append(y)
+        bs, rs = _strides(y)
+        b, M, N = y.shape
+        if b:
+            entries.append((y.data_ptr(), out.data_ptr(), 0, bs, M * N, rs, N, M, N, b, 0.0, 0.0, 0))
+        out = out.view(t.shape[:-2] + (M, N))
+        outs.append(out.mT if swap else out)
+    if entries:
+        lib = L.lib()
+        a, b, c = (L.c_float(v) for v in coefficients)
+
+        def call(mats, n, code, ws, need):
+            L.check(lib.wgs_orthogonalise(mats, n, code, int(steps), a, b, c, L.c_float(eps), ws, need, L.stream()), 'wgs_orthogonalise')
+        if not 1 <= int(steps) <= 16:
+            raise L.WgsError("steps must be 1 .. 16, got %s" % (steps,))
+        _run_matrices(entries, lib.wgs_orthogonalise_ws_bytes, call, xs[0].dtype, xs[0].device, int(steps))
+    return outs if many else outs[0]
+
+
+def _matrix_view(t):
+    """A weight as a dense matrix [first dimension, the rest] in MEMORY order of the rest (2-D: as it is): a convolution's [Co, Ci, kh, kw] in
+    either layout.  A column permutation commutes with the orthogonalisation, so the order does not matter as long as the weight, its gradient and
+    its momentum have the same.  None: no such view."""
+    if t.dim() == 2:
+        return t
+    if t.dim() > 2 and t.is_contiguous():
+        return t.view(t.shape[0], -1)
+    if t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last):
+        return t.permute(0, 2, 3, 1).reshape(t.shape[0], -1)
+    return None
+
+
+@torch.no_grad()
+def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, grad_scale=1.0, steps=5,
+              coefficients=NS_COEFFICIENTS, eps=1e-7):
+    """One update of many matrices in place, in the launches of one:
+
+        momentum buffer  m <- momentum m + g,        u = g + momentum m (nesterov) or m       (g = grad_scale * gradient)
+        weight           W <- (1 - lr weight_decay) W - lr f O,   O = orthogonalise(u),   f = sqrt(max(1, M / N)), or `scale` where given
+
+    params, grads: matrices [M, N] (rows may be strided, elements of a row adjacent), or convolution weights [Co, Ci, kh, kw], contiguous or
+    channels-last, taken as [Co, Ci kh kw]; float32, bfloat16 or float16, one type a call.  momenta: float32 of the same shape and order,
+    contiguous.  The stored momentum and the whole update are fp32; weights are rounded once."""
+    if not (len(params) == len(grads) == len(momenta)):
+        raise L.WgsError("muon_step: %d params, %d grads, %d momenta" % (len(params), len(grads), len(momenta)))
+    if not params:
+        return
+    if not 0.0 <= momentum < 1.0:
+        raise L.WgsError("momentum must be in [0, 1), got %s" % (momentum,))
+    if not 1 <= int(steps) <= 16:
+        raise L.WgsError("steps must be 1 .. 16, got %s" % (steps,))
+    dev, dtype = params[0].device, params[0].dtype
+    entries, seen = [], set()
+    decay = 1.0 - lr * weight_decay
+    for w, g, m in zip(params, grads, momenta):
+        _check_matrix(w, 'param', dev, dtype)
+        _check_matrix(g, 'grad', dev, dtype)
+        if m.dtype != torch.float32 or m.device != dev or m.shape != w.shape or g.shape != w.shape:
+            raise L.WgsError("a momentum must be float32 of its param's shape on its device, got %s %s on %s and grad %s for param %s" % (
+                m.dtype, tuple(m.shape), m.device, tuple(g.shape), tuple(w.shape)))
+        if w.dim() != 2 and not (w.stride() == m.stride() == g.stride()):
+            raise L.WgsError("a convolution weight, its gradient and its momentum must have the same layout, got strides %s %s %s" % (
+                w.stride(), g.stride(), m.stride()))
+        w2, g2, m2 = _matrix_view(w), _matrix_view(g), _matrix_view(m)
+        if w2 is None or g2 is None or m2 is None:
+            raise L.WgsError("muon_step takes matrices and dense convolution weights, got shape %s strides %s" % (tuple(w.shape), w.stride()))
+        M, N = w2.shape
+        if not m2.is_contiguous():
+            raise L.WgsError("momentum must be contiguous")
+        for t, what in ((w2, 'param'), (g2, 'grad')):
+            if (N > 1 and t.stride(1) != 1) or (M > 1 and t.stride(0) < N):
+                raise L.WgsError("%s: the elements of a row must be adjacent, got strides %s" % (what, t.stride()))
+        if w2.data_ptr() in seen or m2.data_ptr() in seen:
+            raise L.WgsError("muon_step: a param or momentum is given twice")
+        seen.add(w2.data_ptr())
+        seen.add(m2.data_ptr())
+        f = max(1.0, M / N) ** 0.5 if scale is None else scale
+        gr, wr = (g2.stride(0), w2.stride(0)) if M > 1 else (N, N)
+        entries.append((g2.data_ptr(), w2.data_ptr(), m2.data_ptr(), 0, 0, gr, wr, M, N, 1, lr * f, decay, 0))
+    lib = L.lib()
+    a, b, c = (L.c_float(v) for v in coefficients)
+
+    def call(mats, n, code, ws, need):
+        L.check(lib.wgs_muon_step(mats, n, code, L.c_float(momentum), int(bool(nesterov)), L.c_float(grad_scale), int(steps), a, b, c, L.c_float(eps),
+                                  ws, need, L.stream()), 'wgs_muon_step')
+    _run_matrices(entries, lib.wgs_muon_step_ws_bytes, call, dtype, dev, int(steps))
