@@ -15,12 +15,14 @@
 #include "wgs_common.h"
 #include "../../include/wgs.h"
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int frag __attribute__((ext_vector_type(4)));      // half8 in storage (vectors of halves are kept one half a register across branches)
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
 constexpr int MAX_MATS = 24;             // matrices of one launch (they travel as kernel arguments)
@@ -28,6 +30,11 @@ constexpr int MAX_STEPS = 16;
 constexpr int INFO = 64;                 // floats of an instance's scalars: f0, then sA[t], sX[t]
 constexpr int I_SA = 4, I_SX = I_SA + MAX_STEPS + 1;
 constexpr int STAT_BLOCKS = 256;         // partial norms of an instance
+// Long sums over few 64 x 64 tiles are split over workgroups, at least SPLIT_NK chunks each: the parts go to the workspace, and a second launch adds
+// them, in order, and does the epilogue.  (One launch whose last workgroup a tile adds the parts was slower: the fence that makes them visible
+// between XCDs writes back a whole L2, some hundred times.)
+constexpr int SPLIT_NK = 12, SPLIT_ITEMS = 1024;
+constexpr int64_t SPLIT_BYTES = (int64_t)SPLIT_ITEMS * 64 * 64 * 4;
 constexpr int BK = 32, ROW = 64;         // K values (bytes) of an LDS row
 constexpr int OOB = (int)0x80000000;     // byte offset behind every plane: the load gives zeros
 
@@ -42,12 +49,14 @@ struct Mat {
     float step, decay;       // step only: W <- decay W - step O
 };
 struct Group {
-    Mat mat[MAX_MATS];
     unsigned char* ws;
     int count, instances;
     int npx, nt, ns;         // planes of X / X^T, buffers of X^T, m x m buffers
     int stat_blocks;
     int dtype, step;         // element type of in / out; a weight update rather than the bare factor
+    int64_t info;            // byte offset of the scalars, INFO floats an instance
+    int64_t part;            // byte offset of the partial tiles of split sums (0: none)
+    Mat mat[MAX_MATS];
 };
 // dimensions of an entry's planes
 struct Dims {
@@ -78,13 +87,9 @@ __device__ __forceinline__ Plane plane_of(const Group& g, const Mat& a, const Di
 }
 // header of the workspace: partial norms, then the scalars of every instance
 struct Part { double ss; float amax; float pad; };
-__host__ __device__ __forceinline__ int64_t header_bytes(int instances, int blocks) {
-    return up((int64_t)instances * blocks * (int64_t)sizeof(Part), 256) + up((int64_t)instances * INFO * 4, 256);
-}
 __device__ __forceinline__ Part* parts_of(const Group& g, int inst) { return (Part*)g.ws + (int64_t)inst * g.stat_blocks; }
-__device__ __forceinline__ float* info_of(const Group& g, int inst) {
-    return (float*)(g.ws + up((int64_t)g.instances * g.stat_blocks * (int64_t)sizeof(Part), 256)) + (int64_t)inst * INFO;
-}
+__device__ __forceinline__ float* info_of(const Group& g, int inst) { return (float*)(g.ws + g.info) + (int64_t)inst * INFO; }
+__host__ __device__ __forceinline__ int parts_of_sum(int nk, int most) { const int s = nk / SPLIT_NK; return s < 1 ? 1 : (s < most ? s : most); }
 // instance -> its entry (a scalar search over at most MAX_MATS entries)
 __device__ __forceinline__ int entry_of(const Group& g, int inst) {
     int e = 0;
@@ -105,6 +110,20 @@ __device__ __forceinline__ void store_as(int dt, void* p, int64_t i, float v) {
     else if (dt == WGS_BF16) ((__bf16*)p)[i] = (__bf16)v;
     else ((_Float16*)p)[i] = (_Float16)v;
 }
+// 16 bytes -> 4 (fp32) or 8 floats
+template <int DT> __device__ __forceinline__ void unpack_as(uint4 q, float* v) {
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (DT == WGS_F32) v[i] = __uint_as_float(w[i]);
+        else if (DT == WGS_BF16) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+        else {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            const h2 h = __builtin_bit_cast(h2, w[i]);
+            v[2 * i] = (float)h[0]; v[2 * i + 1] = (float)h[1];
+        }
+    }
+}
 // The update that is orthogonalised.  STEP: momentum <- mu momentum + g, u = g + mu momentum (nesterov) or momentum.
 struct Momentum { float mu, grad_scale; int nesterov; };
 template <int DT, bool STEP>
@@ -120,32 +139,82 @@ __device__ __forceinline__ float update_of(const Mat& a, int64_t i, int64_t mi, 
 }
 
 // ---- 1. partial norms (and the new momentum) ----------------------------------------------------------------------------------------
+// Memory-bound: 16-byte loads, four in flight, where the matrix is dense and aligned (one element at a time otherwise).  Squares are summed in
+// fp64: neither 1e30 nor 1e-30 leaves its range.
 template <int DT, bool STEP>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const Group g, const Momentum mo) {
-    __shared__ double rs[4];
-    __shared__ float rm[4];
-    const int inst = blockIdx.x / (unsigned)g.stat_blocks, blk = blockIdx.x % (unsigned)g.stat_blocks;
+__global__ __launch_bounds__(512) void ortho_norm_kernel(const Group g, const Momentum mo) {
+    constexpr int V = DT == WGS_F32 ? 4 : 8;
+    __shared__ double rs[8];
+    __shared__ float rm[8];
+    const int inst = blockIdx.x / (unsigned)g.stat_blocks, blk = blockIdx.x % (unsigned)g.stat_blocks, t = threadIdx.x;
     const Mat& a = g.mat[entry_of(g, inst)];
     const int b = inst - a.first;
     const int64_t total = (int64_t)a.M * a.N, off = b * a.in_bs, moff = b * total;
-    const int64_t per = up((total + g.stat_blocks - 1) / g.stat_blocks, 1024);
+    const int64_t per = up((total + g.stat_blocks - 1) / g.stat_blocks, 512 * V);
     const int64_t e0 = blk * per, e1 = e0 + per < total ? e0 + per : total;
     double ss = 0.0;
     float amax = 0.f;
-    for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
+    auto take = [&](float v) { ss = __builtin_fma((double)v, (double)v, ss); amax = fmaxf(amax, fabsf(v)); };
+    int64_t tail = e0;
+    const bool dense = a.in_rs == a.N && ((uintptr_t)a.in & 15) == 0 && off % V == 0 && (!STEP || (((uintptr_t)a.momentum & 15) == 0 && moff % 4 == 0));
+    if (dense) {
+        const int64_t n = e1 > e0 ? (e1 - e0) / V : 0;
+        const uint4* src = (const uint4*)((const char*)a.in + (off + e0) * (DT == WGS_F32 ? 4 : 2));
+        float4* mom = STEP ? (float4*)(a.momentum + moff + e0) : nullptr;
+        constexpr int U = STEP ? 2 : 4;
+        for (int64_t i0 = 0; i0 < n; i0 += 512 * U) {
+            uint4 q[U];
+            float4 m[U][V / 4];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t i = i0 + u * 512 + t;
+                q[u] = make_uint4(0, 0, 0, 0);
+                if (i < n) {
+                    q[u] = src[i];
+                    if (STEP)
+#pragma unroll
+                        for (int w = 0; w < V / 4; ++w) m[u][w] = mom[i * (V / 4) + w];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t i = i0 + u * 512 + t;
+                if (i >= n) continue;
+                float v[V];
+                unpack_as<DT>(q[u], v);
+                if (STEP) {
+#pragma unroll
+                    for (int w = 0; w < V / 4; ++w) {
+                        float* x = &m[u][w].x;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float gr = v[4 * w + k] * mo.grad_scale;
+                            x[k] = __builtin_fmaf(mo.mu, x[k], gr);
+                            v[4 * w + k] = mo.nesterov ? __builtin_fmaf(mo.mu, x[k], gr) : x[k];
+                        }
+                        mom[i * (V / 4) + w] = m[u][w];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < V; ++k) take(v[k]);
+            }
+        }
+        tail = e0 + n * V;
+    }
+    for (int64_t e = tail + t; e < e1; e += 512) {
         const int64_t i = a.in_rs == a.N ? e : (e / a.N) * a.in_rs + e % a.N;
-        const float v = update_of<DT, STEP>(a, off + i, moff + e, mo, true);
-        ss += (double)v * v;
-        amax = fmaxf(amax, fabsf(v));
+        take(update_of<DT, STEP>(a, off + i, moff + e, mo, true));
     }
     ss = wave_sum_d(ss);
     amax = wave_max(amax);
-    if ((threadIdx.x & 63) == 0) { rs[threadIdx.x >> 6] = ss; rm[threadIdx.x >> 6] = amax; }
+    if ((t & 63) == 0) { rs[t >> 6] = ss; rm[t >> 6] = amax; }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (t == 0) {
+        double x = 0.0;
+        float y = 0.f;
+        for (int w = 0; w < 8; ++w) { x += rs[w]; y = fmaxf(y, rm[w]); }
         Part* p = parts_of(g, inst) + blk;
-        p->ss = rs[0] + rs[1] + rs[2] + rs[3];
-        p->amax = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
+        p->ss = x; p->amax = y;
     }
 }
 
@@ -159,8 +228,39 @@ __device__ __forceinline__ float pow2_under(float bound, int top, int lo, int hi
     return ldexpf(1.f, s);
 }
 __device__ __forceinline__ void split_pair(float v, _Float16& h, _Float16& l) {
+    asm volatile("" : "+v"(v));              // the value as rounded to fp32: a product may not be fused into one of the two conversions alone
     h = (_Float16)v;
     l = (_Float16)(v - (float)h);
+}
+// N values at once, two a conversion (to nearest)
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+template <int N, typename V> __device__ __forceinline__ void split_many(const float* v, V& h, V& l) {
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+        float2v x = {v[k], v[k + 1]};
+        asm volatile("" : "+v"(x));
+        const half2v p = __builtin_convertvector(x, half2v);
+        const float2v r = {__builtin_fmaf((float)p[0], -1.f, x[0]), __builtin_fmaf((float)p[1], -1.f, x[1])};
+        const half2v q = __builtin_convertvector(r, half2v);
+        h[k] = p[0]; h[k + 1] = p[1]; l[k] = q[0]; l[k + 1] = q[1];
+    }
+}
+// the input's own power of two: its largest entry between 2^14 and 2^15
+__device__ __forceinline__ float scale_of(double ss, float amax) { return (ss < 1e300 && amax > 0.f) ? pow2_under(amax, 15, -120, 120) : 1.f; }
+// the scalars of an instance from its sum of squares and largest entry
+__device__ __forceinline__ void write_info(float* info, double ss, float amax, float mult, int n, const Bounds& bd) {
+    const bool finite = ss < 1e300;          // false for NaN and infinity: NaN throughout
+    const double inv = ss > 0.0 ? 1.0 / (sqrt(ss) + (double)bd.eps) : 0.0;
+    info[0] = finite ? (float)(inv / (double)mult) : NAN;
+    const double top = (double)amax * inv;
+    const double d0 = finite ? (double)n * top * top : 1.0;
+    for (int k = 0; k <= bd.steps; ++k) {
+        double v = d0 * (double)bd.grow[k];
+        v = v < (double)bd.cap[k] ? v : (double)bd.cap[k];
+        info[I_SA + k] = pow2_under((float)(v > 1e-30 ? v : 1e-30), 14, -60, 60);
+        info[I_SX + k] = pow2_under((float)sqrt(v > 1e-70 ? v : 1e-70), 14, -60, 110);
+    }
 }
 template <int DT, bool STEP>
 __global__ __launch_bounds__(256) void ortho_split_kernel(const Group g, const Momentum mo, const Bounds bd, int tiles) {
@@ -193,49 +293,368 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(const Group g, const M
     __syncthreads();
     ss = rs[0] + rs[1] + rs[2] + rs[3];
     amax = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
-    const bool finite = ss < 1e300;          // false for NaN and infinity
-    const float mult = (finite && amax > 0.f) ? pow2_under(amax, 15, -120, 120) : 1.f;
-    if (tt == 0 && t == 0) {
-        float* info = info_of(g, inst);
-        const double inv = ss > 0.0 ? 1.0 / (sqrt(ss) + (double)bd.eps) : 0.0;
-        info[0] = finite ? (float)(inv / (double)mult) : NAN;
-        const double top = (double)amax * inv;
-        const double d0 = finite ? (double)d.n * top * top : 1.0;
-        for (int k = 0; k <= bd.steps; ++k) {
-            double v = d0 * (double)bd.grow[k];
-            v = v < (double)bd.cap[k] ? v : (double)bd.cap[k];
-            info[I_SA + k] = pow2_under((float)(v > 1e-30 ? v : 1e-30), 14, -60, 60);
-            info[I_SX + k] = pow2_under((float)sqrt(v > 1e-70 ? v : 1e-70), 14, -60, 110);
-        }
-    }
+    const float mult = scale_of(ss, amax);
+    if (tt == 0 && t == 0) write_info(info_of(g, inst), ss, amax, mult, d.n, bd);
     const int64_t off = b * a.in_bs, moff = (int64_t)b * a.M * a.N;
-    for (int i = t; i < 64 * 64; i += 256) {
-        const int r = r0 + (i >> 6), c = c0 + (i & 63);
-        float v = 0.f;
-        if (r < a.M && c < a.N) v = update_of<DT, STEP>(a, off + (int64_t)r * a.in_rs + c, moff + (int64_t)r * a.N + c, mo, false) * mult;
-        tile[i >> 6][i & 63] = v;
+    const bool vec = r0 + 64 <= a.M && c0 + 64 <= a.N && a.in_rs % 8 == 0 && off % 8 == 0 && ((uintptr_t)a.in & 15) == 0 &&
+                     (!STEP || (a.N % 4 == 0 && moff % 4 == 0 && ((uintptr_t)a.momentum & 15) == 0));
+    if (vec) {
+        constexpr int V = DT == WGS_F32 ? 4 : 8, PER = 64 / V;
+#pragma unroll
+        for (int i = t; i < 64 * PER; i += 256) {
+            const int r = i / PER, c = (i % PER) * V;
+            float v[V];
+            unpack_as<DT>(*(const uint4*)((const char*)a.in + (off + (int64_t)(r0 + r) * a.in_rs + c0 + c) * (DT == WGS_F32 ? 4 : 2)), v);
+            if (STEP) {
+                const float4* m = (const float4*)(a.momentum + moff + (int64_t)(r0 + r) * a.N + c0 + c);
+#pragma unroll
+                for (int w = 0; w < V / 4; ++w) {
+                    const float4 q = m[w];
+                    const float x[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[4 * w + k] = mo.nesterov ? __builtin_fmaf(mo.mu, x[k], v[4 * w + k] * mo.grad_scale) : x[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) tile[r][c + k] = v[k] * mult;
+        }
+    } else {
+        for (int i = t; i < 64 * 64; i += 256) {
+            const int r = r0 + (i >> 6), c = c0 + (i & 63);
+            float v = 0.f;
+            if (r < a.M && c < a.N) v = update_of<DT, STEP>(a, off + (int64_t)r * a.in_rs + c, moff + (int64_t)r * a.N + c, mo, false) * mult;
+            tile[i >> 6][i & 63] = v;
+        }
     }
     __syncthreads();
     const bool wide = a.M <= a.N;
     const Plane nat = plane_of(g, a, d, b, wide ? BUF_X : BUF_T0), tra = plane_of(g, a, d, b, wide ? BUF_T0 : BUF_X);
-    // natural: rows r < M, columns up to the padding; transposed: rows c < N, columns r up to the padding.  Two columns a thread.
-    for (int i = t; i < 64 * 32; i += 256) {
-        const int x = i >> 5, y = (i & 31) * 2;
+    // natural: rows r < M, columns up to the padding; transposed: rows c < N, columns r up to the padding.  Eight columns (16 bytes) a thread;
+    // the padded lengths are multiples of 32.
+    auto put = [&](const Plane& p, int row, int col, const float (&v)[8]) {
+        half8 h, l;
+        split_many<8>(v, h, l);
+        unsigned char* q = p.hi + ((int64_t)row * p.ld + col) * 2;
+        *reinterpret_cast<half8*>(q) = h;
+        if (LO) *reinterpret_cast<half8*>(q + p.step) = l;
+    };
+#pragma unroll
+    for (int i = t; i < 64 * 8; i += 256) {
+        const int x = i >> 3, y = (i & 7) * 8;
+        float v[8];
         if (r0 + x < a.M && c0 + y < nat.ld) {
-            _Float16 h0, l0, h1, l1;
-            split_pair(tile[x][y], h0, l0); split_pair(tile[x][y + 1], h1, l1);
-            const int64_t at = ((int64_t)(r0 + x) * nat.ld + c0 + y) * 2;
-            _Float16* q = (_Float16*)(nat.hi + at);
-            q[0] = h0; q[1] = h1;
-            if (LO) { _Float16* w = (_Float16*)(nat.hi + nat.step + at); w[0] = l0; w[1] = l1; }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = tile[x][y + k];
+            put(nat, r0 + x, c0 + y, v);
         }
         if (c0 + x < a.N && r0 + y < tra.ld) {
-            _Float16 h0, l0, h1, l1;
-            split_pair(tile[y][x], h0, l0); split_pair(tile[y + 1][x], h1, l1);
-            const int64_t at = ((int64_t)(c0 + x) * tra.ld + r0 + y) * 2;
-            _Float16* q = (_Float16*)(tra.hi + at);
-            q[0] = h0; q[1] = h1;
-            if (LO) { _Float16* w = (_Float16*)(tra.hi + tra.step + at); w[0] = l0; w[1] = l1; }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = tile[y + k][x];
+            put(tra, c0 + x, r0 + y, v);
+        }
+    }
+}
+
+// ---- small matrices: everything in one launch -------------------------------------------------------------------------------------------------
+// m <= 32 MT <= 64, n <= SMALL_N: one workgroup a matrix, the m x m matrices in LDS.  X lies in blocks of 32 columns as the operand "lane = column j,
+// 8 rows i": the product's own result layout (lane = column, rows 8 q + 4 half + 0..3) is an operand again once the sum's index is taken in that
+// order, B's fragments being read from LDS in the same one.  The next Gram matrix needs X with lane = row: the transposed product X^T B, from the
+// same two operands, has it, and is used and dropped block by block.  A block's fragments stay with one wave, which stores and loads them lane by
+// lane (1 KB at a time) through the caches: in registers they do not fit beside the accumulators.  The waves' partial Gram matrices are added in
+// a fixed order.  Bound by the latency of its steps and one CU's matrix cores; the many launches of the general path cost more up to these sizes.
+constexpr int SMALL_N = 2048, SMALL_WAVES = 8;
+struct SmallArgs { Bounds bd; float sb[MAX_STEPS]; float a, b, c; };
+__host__ __device__ __forceinline__ bool is_small(const Dims& d) { return d.m <= 64 && d.n <= SMALL_N; }
+__host__ __device__ __forceinline__ int64_t small_bytes(const Dims& d) { return 64 * (int64_t)d.np * 4; }
+template <int MT>
+__global__ __launch_bounds__(64 * SMALL_WAVES, 1) void ortho_small_kernel(const Group g, const Momentum mo, const SmallArgs ar) {
+    constexpr int W = SMALL_WAVES, TRI = MT * (MT + 1) / 2, LD = 32 * MT + 8, TURNS = 16 * MT, U = 16;
+    __shared__ float part[W][TRI][32][33];
+    __shared__ __attribute__((aligned(16))) _Float16 sa[2][32 * MT][LD], sbm[2][32 * MT][LD];
+    __shared__ double rs[W];
+    __shared__ float rm[W];
+    __shared__ float info[INFO];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, lh = lane >> 5;
+    const Mat& mat = g.mat[entry_of(g, blockIdx.x)];
+    const int b = blockIdx.x - mat.first;
+    const Dims d = dims_of(mat.M, mat.N);
+    const bool wide = mat.M <= mat.N;
+    const int64_t off = b * mat.in_bs, moff = (int64_t)b * mat.M * mat.N, ob = b * mat.out_bs;
+    float* tr = &part[wave][0][0][0];          // a wave's own [32 MT rows i][33]
+    const int blocks = d.np / 32, active = blocks < W ? blocks : W;
+    frag* const frags = (frag*)(g.ws + mat.ws + b * small_bytes(d)) + lane;      // block k: [tile][half][hi, lo][64 lanes]
+    auto at = [&](int k, int t, int ks, int pl) { return frags + (((int64_t)k * MT + t) * 4 + ks * 2 + pl) * 64; };
+    auto split = [&](const float* v, frag& fh, frag& fl) {
+        half8 h, l;
+        split_many<8>(v, h, l);
+        fh = __builtin_bit_cast(frag, h); fl = __builtin_bit_cast(frag, l);
+    };
+    auto mul = [](frag x, frag y, f32x16 z) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, y), z, 0, 0, 0); };
+
+    // Element e of block k: lane and turn own it, in the two passes over the input (norm and new momentum first, then the scaled operands, from
+    // the caches) and in the one over the result.  Loads go to clamped addresses, unconditionally: they are in flight together.
+    auto typed = [&](auto f) __attribute__((always_inline)) {
+        if (g.dtype == WGS_F32) f(std::integral_constant<int, WGS_F32>());
+        else if (g.dtype == WGS_BF16) f(std::integral_constant<int, WGS_BF16>());
+        else f(std::integral_constant<int, WGS_F16>());
+    };
+    // A lane's elements of block k: column c of the matrix, rows r0, r0 + dr, ...; in LDS at t0, t0 + dt, ...
+    struct Own { int r0, dr, c, t0, dt; };
+    auto own = [&](int k) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));            // (formed here, not kept in registers through the kernel)
+        const int hi = ln / (32 * MT), lo = ln & (32 * MT - 1);
+        return wide ? Own{ln >> 5, 2, k * 32 + (ln & 31), (ln >> 5) * 33 + (ln & 31), 66} : Own{k * 32 + hi, 2 / MT, lo, lo * 33 + hi, 2 / MT};
+    };
+    auto input = [&](bool first, int k, float mult, auto take) __attribute__((always_inline)) {
+        typed([&](auto dt) __attribute__((always_inline)) {
+            constexpr int DT = decltype(dt)::value;
+            const Own o = own(k);
+            const int cc = o.c < mat.N ? o.c : mat.N - 1;
+#pragma unroll 1
+            for (int it0 = 0; it0 < TURNS; it0 += U) {
+                float v[U], mm[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    int r = o.r0 + (it0 + u) * o.dr;
+                    r = r < mat.M ? r : mat.M - 1;
+                    v[u] = load_elem<DT>(mat.in, off + cc + (int64_t)r * mat.in_rs);
+                    mm[u] = 0.f;
+                    if (g.step) mm[u] = mat.momentum[moff + cc + r * mat.N];
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int r = o.r0 + (it0 + u) * o.dr;
+                    const bool ok = r < mat.M && o.c < mat.N;
+                    if (g.step) {
+                        const float gr = v[u] * mo.grad_scale;
+                        if (first) {
+                            mm[u] = __builtin_fmaf(mo.mu, mm[u], gr);
+                            if (ok) mat.momentum[moff + cc + r * mat.N] = mm[u];
+                        }
+                        v[u] = mo.nesterov ? __builtin_fmaf(mo.mu, mm[u], gr) : mm[u];
+                    }
+                    take(o.t0 + (it0 + u) * o.dt, ok ? v[u] * mult : 0.f);
+                }
+            }
+        });
+    };
+    double ss = 0.0;
+    float amax = 0.f;
+#pragma unroll 1
+    for (int k = wave; k < blocks; k += W)
+        input(true, k, 1.f, [&](int, float v) {
+            ss = __builtin_fma((double)v, (double)v, ss);
+            amax = fmaxf(amax, fabsf(v));
+        });
+    ss = wave_sum_d(ss);
+    amax = wave_max(amax);
+    if (lane == 0) { rs[wave] = ss; rm[wave] = amax; }
+    __syncthreads();
+    ss = 0.0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) { ss += rs[w]; amax = fmaxf(amax, rm[w]); }
+    const float mult = scale_of(ss, amax);
+    if (tid == 0) write_info(info, ss, amax, mult, d.n, ar.bd);
+
+    f32x16 gr[TRI];
+    auto gram = [&](const frag (&ih)[MT][2], const frag (&il)[MT][2]) __attribute__((always_inline)) {       // adds one block: lane = row i, 8 columns a fragment
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int pr = 0; pr < 3; ++pr)
+#pragma unroll
+                for (int t = 0; t < TRI; ++t) {
+                    const int p = t == 0 ? 0 : 1, q = t == 2 ? 1 : 0;
+                    gr[t] = mul(pr == 0 ? il[p][ks] : ih[p][ks], pr == 1 ? il[q][ks] : ih[q][ks], gr[t]);
+                }
+    };
+    auto clear = [&]() {
+#pragma unroll
+        for (int t = 0; t < TRI; ++t)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) gr[t][q] = 0.f;
+    };
+    // the operands, through LDS: lane = column to stay, lane = row for the first Gram matrix
+    clear();
+#pragma unroll 1
+    for (int k = wave; k < blocks; k += W) {
+        asm volatile("" ::: "memory");
+        input(false, k, mult, [&](int i, float v) { tr[i] = v; });
+        asm volatile("" ::: "memory");
+        frag ih[MT][2], il[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            float v[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) v[q] = tr[(32 * t + 8 * (q >> 2) + 4 * lh + (q & 3)) * 33 + l31];
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                frag h, l;
+                split(v + 8 * ks, h, l);
+                *at(k, t, ks, 0) = h; *at(k, t, ks, 1) = l;
+            }
+#pragma unroll
+            for (int q = 0; q < 16; ++q) v[q] = tr[(32 * t + l31) * 33 + 8 * (q >> 2) + 4 * lh + (q & 3)];
+            split(v, ih[t][0], il[t][0]);
+            split(v + 8, ih[t][1], il[t][1]);
+        }
+        gram(ih, il);
+    }
+#pragma unroll 1
+    for (int t = 0; t < ar.bd.steps; ++t) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid) :: "memory");       // (nor the LDS addresses from step to step)
+        const int lane = tid & 63, l31 = lane & 31, lh = lane >> 5;
+        if (wave < active)
+#pragma unroll
+            for (int k = 0; k < TRI; ++k)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) part[wave][k][8 * (q >> 2) + 4 * lh + (q & 3)][l31] = gr[k][q];
+        __syncthreads();
+        const float fx = t == 0 ? info[0] : 1.f / info[I_SX + t], sA = info[I_SA + t], ga = fx * fx * sA;
+#pragma unroll
+        for (int it = 0; it < TRI * 1024 / (64 * W); ++it) {
+            const int e = it * 64 * W + tid, k = e >> 10, r = (e >> 5) & 31, c = e & 31;
+            const int p = k == 0 ? 0 : 1, q = k == 2 ? 1 : 0;
+            if (p == q && r < c) continue;
+            float v = part[0][k][r][c];
+            for (int w = 1; w < active; ++w) v += part[w][k][r][c];
+            _Float16 h, l;
+            split_pair(v * ga, h, l);
+            sa[0][32 * p + r][32 * q + c] = h; sa[1][32 * p + r][32 * q + c] = l;
+            sa[0][32 * q + c][32 * p + r] = h; sa[1][32 * q + c][32 * p + r] = l;
+        }
+        __syncthreads();
+        if (wave < TRI) {
+            const int p = wave == 0 ? 0 : 1, q = wave == 2 ? 1 : 0;
+            f32x16 s0, s1;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) { s0[k] = 0.f; s1[k] = 0.f; }
+#pragma unroll
+            for (int ks = 0; ks < 2 * MT; ++ks) {
+                const int kc = 16 * ks + 8 * lh;
+                const half8 ah = *reinterpret_cast<const half8*>(&sa[0][32 * p + l31][kc]), al = *reinterpret_cast<const half8*>(&sa[1][32 * p + l31][kc]);
+                const half8 bh = *reinterpret_cast<const half8*>(&sa[0][32 * q + l31][kc]), bl = *reinterpret_cast<const half8*>(&sa[1][32 * q + l31][kc]);
+                s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, s0, 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, s1, 0, 0, 0);
+                s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, s0, 0, 0, 0);
+            }
+            const float isa = 1.f / sA;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int r = 8 * (k >> 2) + 4 * lh + (k & 3), c = l31;
+                const float A = ((float)sa[0][32 * p + r][32 * q + c] + (float)sa[1][32 * p + r][32 * q + c]) * isa;
+                const float v = ((p == q && r == c ? ar.a : 0.f) + (ar.b * A + ar.c * ((s0[k] + s1[k]) * isa * isa))) * ar.sb[t];
+                _Float16 h, l;
+                split_pair(v, h, l);
+                if (p != q || r >= c) {
+                    sbm[0][32 * p + r][32 * q + c] = h; sbm[1][32 * p + r][32 * q + c] = l;
+                    sbm[0][32 * q + c][32 * p + r] = h; sbm[1][32 * q + c][32 * p + r] = l;
+                }
+            }
+        }
+        __syncthreads();
+        const bool last = t + 1 == ar.bd.steps;
+        const float fo = last ? fx / ar.sb[t] : fx * info[I_SX + t + 1] / ar.sb[t];
+        clear();
+        frag nh[MT][2], nl[MT][2];               // the next block's fragments
+        auto load = [&](int k) {
+#pragma unroll
+            for (int u = 0; u < MT; ++u)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) { nh[u][ks] = *at(k, u, ks, 0); nl[u][ks] = *at(k, u, ks, 1); }
+        };
+        if (wave < blocks) load(wave);
+#pragma unroll 1
+        for (int k = wave; k < blocks; k += W) {
+            frag vh[MT][2], vl[MT][2];
+#pragma unroll
+            for (int u = 0; u < MT; ++u)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) { vh[u][ks] = nh[u][ks]; vl[u][ks] = nl[u][ks]; }
+            load(k + W < blocks ? k + W : k);
+            // B X (lane = column) and, from the same operands in the other order, X^T B (lane = row)
+            f32x16 dd[MT], de[MT];
+#pragma unroll
+            for (int u = 0; u < MT; ++u)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) { dd[u][q] = 0.f; de[u][q] = 0.f; }
+            asm volatile("" ::: "memory");          // (B's fragments are read again for every block: kept, they would not fit)
+#pragma unroll
+            for (int ks = 0; ks < 2 * MT; ++ks) {
+                const int kb = 16 * ks + 4 * lh;
+                frag bh[MT], bl[MT];
+#pragma unroll
+                for (int u = 0; u < MT; ++u) {
+                    const int2 h0 = *reinterpret_cast<const int2*>(&sbm[0][32 * u + l31][kb]), h1 = *reinterpret_cast<const int2*>(&sbm[0][32 * u + l31][kb + 8]);
+                    const int2 l0 = *reinterpret_cast<const int2*>(&sbm[1][32 * u + l31][kb]), l1 = *reinterpret_cast<const int2*>(&sbm[1][32 * u + l31][kb + 8]);
+                    bh[u] = frag{h0.x, h0.y, h1.x, h1.y};
+                    bl[u] = frag{l0.x, l0.y, l1.x, l1.y};
+                }
+                const frag ph = vh[ks >> 1][ks & 1], pl = vl[ks >> 1][ks & 1];
+#pragma unroll
+                for (int pr = 0; pr < 3; ++pr)
+#pragma unroll
+                    for (int u = 0; u < MT; ++u) {
+                        const frag x = pr == 0 ? pl : ph, y = pr == 1 ? bl[u] : bh[u];
+                        dd[u] = mul(x, y, dd[u]);
+                        if (!last) de[u] = mul(y, x, de[u]);
+                    }
+            }
+            if (last) {
+                // lane = row i: to LDS as [i][j], then out in rows of the result
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int u = 0; u < MT; ++u)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) tr[(32 * u + l31) * 33 + 8 * (q >> 2) + 4 * lh + (q & 3)] = dd[u][q] * fo;
+                asm volatile("" ::: "memory");
+                typed([&](auto dt) __attribute__((always_inline)) {
+                    constexpr int DT = decltype(dt)::value;
+                    const Own o = own(k);
+                    const int cc = o.c < mat.N ? o.c : mat.N - 1;
+#pragma unroll 1
+                    for (int it0 = 0; it0 < TURNS; it0 += U) {
+                        float w[U];
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            int r = o.r0 + (it0 + u) * o.dr;
+                            r = r < mat.M ? r : mat.M - 1;
+                            w[u] = 0.f;
+                            if (g.step) w[u] = load_elem<DT>(mat.out, ob + cc + (int64_t)r * mat.out_rs);
+                        }
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            const int r = o.r0 + (it0 + u) * o.dr;
+                            float v = tr[o.t0 + (it0 + u) * o.dt];
+                            if (g.step) v = mat.decay * w[u] - mat.step * v;
+                            if (r < mat.M && o.c < mat.N) store_as(DT, mat.out, ob + cc + (int64_t)r * mat.out_rs, v);
+                        }
+                    }
+                });
+                continue;
+            }
+            frag ih[MT][2], il[MT][2];
+            float v[16];
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) v[q] = dd[u][q] * fo;
+                split(v, ih[u][0], il[u][0]); split(v + 8, ih[u][1], il[u][1]);
+            }
+            gram(ih, il);
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) v[q] = de[u][q] * fo;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    frag h, l;
+                    split(v + 8 * ks, h, l);
+                    *at(k, u, ks, 0) = h; *at(k, u, ks, 1) = l;
+                }
+            }
         }
     }
 }
@@ -252,7 +671,7 @@ struct Job {
     float mul;               // factor known on the host
     float a, b, c;           // POLY
 };
-struct Jobs { Job job[2]; int count; int sym; };
+struct Jobs { Job job[2]; int count; int sym; int kgram; };      // kgram: sums over the n columns, not over m
 
 // tile number -> tile coordinates, in squares of 4 x 4 tiles: the tiles that run side by side on an XCD share operands in its L2
 __device__ __forceinline__ void tile_full(int t, int tm, int tn, int& ti, int& tj) {
@@ -276,20 +695,24 @@ __device__ __forceinline__ void tile_lower(int t, int tm, int& ti, int& tj) {
     }
 }
 
-template <int NA, int NB, int BM, int WAVES_M, int WAVES_N, int NS>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(const Group g, const Jobs js, int total) {
+// E: side of the square blocks in which a wave hands its results through LDS to the stores (32 / 64 / 96)
+template <int NA, int NB, int BM, int WAVES_M, int WAVES_N, int NS, int E, bool SPLIT = false>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(const Jobs js, int total, int run, int most, int join, const Group g) {
     constexpr int BN = BM, NW = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 32, TN = WN / 32;
     constexpr int A_BYTES = BM * ROW, B_BYTES = BN * ROW, STAGE = NA * A_BYTES + NB * B_BYTES;
     constexpr int AI = BM / 16 / NW, BI = BN / 16 / NW, NPIECE = NA * AI + NB * BI;
     static_assert(AI * 16 * NW == BM && BI * 16 * NW == BN && TM * 32 * WAVES_M == BM && TN * 32 * WAVES_N == BN, "tile / wave count mismatch");
+    static_assert(WM % E == 0 && WN % E == 0, "epilogue block");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
 
-    // workgroups go round the 8 XCDs: each gets a contiguous range of tiles
-    const int per_xcd = (total + 7) >> 3;
-    int tile = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per_xcd || tile >= total) return;
+    // Workgroups go round the 8 XCDs: runs of at most 32 tiles in turn, equally many each, so that an XCD's CUs work on neighbouring tiles and the
+    // first entries (the longest sums) are spread over all XCDs.
+    const int idx = (int)(blockIdx.x >> 3);
+    int tile = (idx / run * 8 + (int)(blockIdx.x & 7)) * run + idx % run;
+    if (tile >= total) return;
+    int parts = 1, slots = 0, before = 0, slot0 = 0;
     const int half = js.count == 2 ? total / 2 : total;
     const Job& J = js.job[tile >= half ? 1 : 0];
     if (tile >= half) tile -= half;
@@ -298,19 +721,27 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
         const Dims q = dims_of(g.mat[e].M, g.mat[e].N);
         tm = (q.m + BM - 1) / BM; tn = (q.n + BN - 1) / BN;
         per = js.sym ? tm * (tm + 1) / 2 : tm * tn;
+        if (SPLIT) { parts = parts_of_sum((js.kgram ? q.np : q.mp) / BK, most); if (!join) per *= parts; slots = g.mat[e].batch * per * (join ? parts : 1); }
         const int c = g.mat[e].batch * per;
         if (tile < c || e + 1 == g.count) break;
         tile -= c;
+        if (SPLIT) before += slots;
     }
     const Mat& mat = g.mat[e];
     const Dims d = dims_of(mat.M, mat.N);
     const int b = tile / per, inst = mat.first + b;
+    int part = 0;
+    if (SPLIT) {                         // slot of the (first) part in the workspace; parts of a tile are neighbours
+        slot0 = before + (join ? tile * parts : tile);
+        if (!join) { tile -= b * per; part = tile % parts; tile /= parts; per /= parts; tile += b * per; }
+        if (join && parts == 1) return;
+    }
     int ti, tj;
     if (js.sym) tile_lower(tile % per, tm, ti, tj);
     else tile_full(tile % per, tm, tn, ti, tj);
     const int i0 = ti * BM, j0 = tj * BN;
     const Plane P = plane_of(g, mat, d, b, J.p), R = plane_of(g, mat, d, b, J.r);
-    const int nk = P.ld / BK;
+    const int nk_all = P.ld / BK, k0 = SPLIT ? nk_all * part / parts : 0, nk = SPLIT ? nk_all * (part + 1) / parts - k0 : nk_all;
 
     const __amdgpu_buffer_rsrc_t rp0 = __builtin_amdgcn_make_buffer_rsrc(P.hi, 0, (unsigned)P.bytes, 0x00020000);
     const __amdgpu_buffer_rsrc_t rp1 = __builtin_amdgcn_make_buffer_rsrc(P.hi + (NA > 1 ? P.step : 0), 0, (unsigned)P.bytes, 0x00020000);
@@ -331,23 +762,19 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
         const int row = (wave * BI + j) * 16 + lrow, lc = slot ^ ((row >> 2) & 3);
         b_off[j] = j0 + row < rows_r ? (int)(((int64_t)(j0 + row) * R.ld + lc * 8) * 2) : OOB;
     }
+    // piece x of the next chunk (chunk nC, behind the last one that one again: its data is not used) into stage buf
     int nC = 0;
-    auto issue = [&](int buf) {
-        const bool past = nC >= nk;
-        const int adv = past ? 0 : nC * ROW;
-        ++nC;
-#pragma unroll
-        for (int idx = 0; idx < NPIECE; ++idx) {
-            lds_byte* st = (lds_byte*)(smem + buf * STAGE);
-            if (idx < NA * AI) {
-                const int j = idx / NA, pl = idx % NA;
-                const int off = past ? OOB : (int)((unsigned)a_off[j] + (unsigned)adv);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(pl ? rp1 : rp0, st + (wave * AI + j) * 16 * ROW + pl * A_BYTES, 16, off, 0, 0, 0);
-            } else {
-                const int j = (idx - NA * AI) / NB, pl = (idx - NA * AI) % NB;
-                const int off = past ? OOB : (int)((unsigned)b_off[j] + (unsigned)adv);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(pl ? rr1 : rr0, st + NA * A_BYTES + (wave * BI + j) * 16 * ROW + pl * B_BYTES, 16, off, 0, 0, 0);
-            }
+    auto piece = [&](int buf, int x) {
+        const int adv = (k0 + (nC < nk ? nC : nk - 1)) * ROW;
+        lds_byte* st = (lds_byte*)(smem + buf * STAGE);
+        if (x < NA * AI) {
+            const int j = x / NA, pl = x % NA;
+            const int off = a_off[j];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(pl ? rp1 : rp0, st + (wave * AI + j) * 16 * ROW + pl * A_BYTES, 16, off, adv, 0, 0);
+        } else {
+            const int j = (x - NA * AI) / NB, pl = (x - NA * AI) % NB;
+            const int off = b_off[j];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(pl ? rr1 : rr0, st + NA * A_BYTES + (wave * BI + j) * 16 * ROW + pl * B_BYTES, 16, off, adv, 0, 0);
         }
     };
 
@@ -360,46 +787,42 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
     const int l31 = lane & 31, lh = lane >> 5, swz = (l31 >> 2) & 3;
     const int a_rd = (wm * WM + l31) * ROW, b_rd = NA * A_BYTES + (wn * WN + l31) * ROW;
-
-#pragma unroll
-    for (int s = 0; s < NS - 1; ++s) issue(s);
-    int cur = 0, nxt = NS - 1;
-    for (int kt = 0; kt < nk; ++kt) {
-        asm volatile("s_waitcnt vmcnt(%0)" :: "n"((NS - 2) * NPIECE) : "memory");      // this wave's pieces of chunk kt have landed
+    struct Frags { half8 a[TM][NA], b[TN][NB]; };
+    constexpr int READS = TM * NA + TN * NB, PRODS = (NA > 1) + (NB > 1) + 1, MMAS = PRODS * TM * TN;
+    auto read = [&](int buf, int ks, int x, Frags& f) {      // fragment x of half ks of a chunk
+        const unsigned char* base = smem + buf * STAGE + ((2 * ks + lh) ^ swz) * 16;
+        if (x < TM * NA) f.a[x / NA][x % NA] = *reinterpret_cast<const half8*>(base + a_rd + (x % NA) * A_BYTES + (x / NA) * 32 * ROW);
+        else { const int y = x - TM * NA; f.b[y / NB][y % NB] = *reinterpret_cast<const half8*>(base + b_rd + (y % NB) * B_BYTES + (y / NB) * 32 * ROW); }
+    };
+    // The products of one half chunk, small terms first and neighbours on different accumulators, with the reads of the next half's fragments and
+    // the loads of a later chunk spread between them: the matrix pipe is never without a product that is ready.
+#define ORTHO_MMA(F, G2, BUF, KS, LOADS, LBUF)                                                                                              \
+    _Pragma("unroll") for (int n = 0; n < MMAS; ++n) {                                                                                      \
+        constexpr int SIDE = READS + LOADS * NPIECE;                                                                                        \
+        const int pr = PRODS == 3 ? n / (TM * TN) : PRODS == 2 ? 2 * (n / (TM * TN)) : 2, i = (n % (TM * TN)) / TN, j = n % TN;               \
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(F.a[i][pr == 0 ? NA - 1 : 0], F.b[j][pr == 1 ? NB - 1 : 0], acc[i][j], 0, 0, 0);  \
+        _Pragma("unroll") for (int s = n * SIDE / MMAS; s < (n + 1) * SIDE / MMAS; ++s) {                                                   \
+            if (s < READS) read(BUF, KS, s, G2);                                                                                            \
+            else piece(LBUF, s - READS);                                                                                                    \
+        }                                                                                                                                   \
+        __builtin_amdgcn_sched_barrier(0);                                                                                                  \
+    }
+    auto landed = [&](auto left) {       // all chunks in flight but the newest `left` are complete, in every wave, and so are all reads
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(decltype(left)::value * NPIECE) : "memory");
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();                                                   // ... and everybody's; stage nxt is no longer read
+        __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        issue(nxt);
-        const unsigned char* base = smem + cur * STAGE;
+    };
+    // Fragments are read one half chunk ahead of their products; the barrier sits between the two halves, behind products already issued, and
+    // frees the stage whose second half has just been read: its refill has NS - 1 chunks of products to arrive in.
+    Frags f0, f1;
+    if (!SPLIT || !join)
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const int kc = ((2 * ks + lh) ^ swz) * 16;
-            half8 af[TM][NA], bf[TN][NB];
+    for (int s = 0; s < NS; ++s, ++nC)
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int pl = 0; pl < NA; ++pl) af[i][pl] = *reinterpret_cast<const half8*>(base + a_rd + pl * A_BYTES + i * 32 * ROW + kc);
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int pl = 0; pl < NB; ++pl) bf[j][pl] = *reinterpret_cast<const half8*>(base + b_rd + pl * B_BYTES + j * 32 * ROW + kc);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    if (NA > 1) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[i][NA - 1], bf[j][0], acc[i][j], 0, 0, 0);
-                    if (NB > 1) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[i][0], bf[j][NB - 1], acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[i][0], bf[j][0], acc[i][j], 0, 0, 0);
-                }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        cur = cur + 1 == NS ? 0 : cur + 1;
-        nxt = nxt + 1 == NS ? 0 : nxt + 1;
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // the zero loads past the last chunk
-
-    // ---- epilogue: a lane holds column j = lane & 31 and rows 8 q + 4 (lane >> 5) + 0..3 of every 32 x 32 block
+        for (int x = 0; x < NPIECE; ++x) piece(s, x);
+    // the scalars of the epilogue, fetched behind the first loads
     const float* info = info_of(g, inst);
     const float fx = J.first ? info[0] : 1.f / info[I_SX + J.t];
     float mult = J.mul;
@@ -408,22 +831,105 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
     else if (J.kind == PROD_A) mult = J.mul * (info[I_SA + J.t2] / info[I_SA + J.t]);
     else if (J.kind == APPLY_MID) mult = J.mul * fx * info[I_SX + J.t2];
     else if (J.kind == APPLY_OUT) mult = J.mul * fx;
+    const float isa = J.kind == POLY ? 1.f / info[I_SA + J.t] : 0.f;
+    if (!SPLIT || !join) {
+        landed(std::integral_constant<int, NS - 1>());
+#pragma unroll
+        for (int x = 0; x < READS; ++x) read(0, 0, x, f0);
+    }
+    int cur = 0;
+    for (int kt = 0; kt < (SPLIT && join ? 0 : nk); ++kt) {
+        ORTHO_MMA(f0, f1, cur, 1, 0, 0)
+        landed(std::integral_constant<int, NS - 2>());
+        const int old = cur;
+        cur = cur + 1 == NS ? 0 : cur + 1;
+        ORTHO_MMA(f1, f0, cur, 0, 1, old)      // (behind the last chunk the fragments read are not used)
+        ++nC;
+    }
+#undef ORTHO_MMA
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // the loads behind the last chunk: the LDS is used again below
+    __syncthreads();
+    if constexpr (SPLIT) {
+        static_assert(TM == 1 && TN == 1, "one block a wave");
+        float* slot = (float*)(g.ws + g.part) + (int64_t)slot0 * (BM * BN) + (wave * 256 + lane) * 4;
+        if (parts > 1 && !join) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4*>(slot + q * 256) = make_float4(acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]);
+            return;
+        }
+        if (join)
+#pragma unroll 4
+            for (int s = 0; s < parts; ++s)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 v = *reinterpret_cast<const float4*>(slot + (int64_t)s * (BM * BN) + q * 256);
+                    acc[0][0][4 * q] += v.x; acc[0][0][4 * q + 1] += v.y; acc[0][0][4 * q + 2] += v.z; acc[0][0][4 * q + 3] += v.w;
+                }
+    }
+
+    // ---- epilogue: a lane holds column lane & 31 and rows 8 q + 4 (lane >> 5) + 0..3 of every 32 x 32 block.  A wave puts E x E results into its
+    // own part of the LDS and reads them back in rows of either orientation: 16-byte stores over whole cache lines.
+    constexpr int LDH = 2 * E + 8;                    // bytes of an fp16 row in LDS (E rows of each plane)
+    constexpr int LDF = E + 4;                        // floats of an fp32 row in LDS
+    unsigned char* mine = smem + wave * (E * LDF * 4);
+    static_assert(2 * E * LDH == E * LDF * 4, "one region for both forms");
+    auto fence = [&]() { asm volatile("" ::: "memory"); };      // a wave's LDS operations execute in order
+
     if (J.kind == APPLY_OUT) {
-        const bool wide = mat.M <= mat.N;
+        const bool wide = mat.M <= mat.N;             // rows of the result are rows of X, or of X^T
         const int64_t ob = b * mat.out_bs;
+        const int size = g.dtype == WGS_F32 ? 4 : 2;
+        const bool vec = mat.out_rs % 4 == 0 && ob % 4 == 0 && ((uintptr_t)mat.out & (4 * size - 1)) == 0;
+        const int rows = wide ? d.m : d.n, cols = wide ? d.n : d.m;
+        float* lds = reinterpret_cast<float*>(mine);
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int bi = 0; bi < WM / E; ++bi)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                const int c = j0 + wn * WN + j * 32 + l31;
+            for (int bj = 0; bj < WN / E; ++bj) {
+                fence();
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                    const int r = i0 + wm * WM + i * 32 + 8 * (q >> 2) + 4 * lh + (q & 3);
-                    if (r < d.m && c < d.n) {
-                        const int64_t at = ob + (wide ? (int64_t)r * mat.out_rs + c : (int64_t)c * mat.out_rs + r);
-                        float v = acc[i][j][q] * mult;
-                        if (g.step) v = mat.decay * load_as(g.dtype, mat.out, at) - mat.step * v;
-                        store_as(g.dtype, mat.out, at, v);
+                for (int i = 0; i < E / 32; ++i)
+#pragma unroll
+                    for (int j = 0; j < E / 32; ++j)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const f32x16& v = acc[bi * (E / 32) + i][bj * (E / 32) + j];
+                            const int c = j * 32 + l31, r = i * 32 + 8 * q + 4 * lh;
+                            if (wide) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) lds[(r + k) * LDF + c] = v[4 * q + k] * mult;
+                            } else {
+                                *reinterpret_cast<float4*>(lds + c * LDF + r) = make_float4(v[4 * q] * mult, v[4 * q + 1] * mult, v[4 * q + 2] * mult, v[4 * q + 3] * mult);
+                            }
+                        }
+                fence();
+                const int rb = i0 + wm * WM + bi * E, cb = j0 + wn * WN + bj * E;
+                const int r0 = wide ? rb : cb, c0 = wide ? cb : rb;
+#pragma unroll 4
+                for (int x = lane; x < E * E / 4; x += 64) {
+                    const int r = x / (E / 4), c = (x % (E / 4)) * 4;
+                    const float4 f = *reinterpret_cast<const float4*>(lds + r * LDF + c);
+                    float v[4] = {f.x, f.y, f.z, f.w};
+                    if (r0 + r >= rows || c0 + c >= cols) continue;
+                    const int64_t at = ob + (int64_t)(r0 + r) * mat.out_rs + c0 + c;
+                    const bool full = vec && c0 + c + 4 <= cols;
+                    char* o = (char*)mat.out + at * size;
+                    if (g.step) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (full || c0 + c + k < cols) v[k] = mat.decay * load_as(g.dtype, mat.out, at + k) - mat.step * v[k];
+                    }
+                    if (full) {
+                        if (size == 4) *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+                        else if (g.dtype == WGS_BF16) {
+                            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+                            *reinterpret_cast<b4*>(o) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+                        } else *reinterpret_cast<half4*>(o) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (c0 + c + k < cols) store_as(g.dtype, mat.out, at + k, v[k]);
                     }
                 }
             }
@@ -433,68 +939,97 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
     const Plane D = plane_of(g, mat, d, b, J.dst);                              // [i][j]
     const Plane T = mid ? plane_of(g, mat, d, b, J.dst2) : D;                   // [j][i]
     const Plane S = J.kind == POLY ? plane_of(g, mat, d, b, J.src) : D;
-    const float isa = J.kind == POLY ? 1.f / info[I_SA + J.t] : 0.f;
     const int nc = mid ? d.n : d.m;
+    unsigned char* lo = mine + E * LDH;               // LDS: [c][r] of the hi parts, then of the lo parts
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int bi = 0; bi < WM / E; ++bi)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int c = j0 + wn * WN + j * 32 + l31, rb = i0 + wm * WM + i * 32, cb = j0 + wn * WN + j * 32;
+        for (int bj = 0; bj < WN / E; ++bj) {
+            const int rb = i0 + wm * WM + bi * E, cb = j0 + wn * WN + bj * E;
             // A tile on the diagonal computes both triangles, whose roundings differ where the factors do not quite commute: the strict upper
             // one is dropped, else the iteration amplifies the antisymmetric part (measured: ten times the error on spiked spectra).
             if (!mid && rb < cb) continue;
             const bool half = !mid && rb == cb;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int r = i0 + wm * WM + i * 32 + 8 * q + 4 * lh;
-                float v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = acc[i][j][4 * q + k] * mult;
-                if (J.kind == POLY) {
-                    if (c < d.m && r < d.mp) {
-                        const half4 sh = *reinterpret_cast<const half4*>(S.hi + ((int64_t)c * S.ld + r) * 2);
-                        const half4 sl = *reinterpret_cast<const half4*>(S.hi + S.step + ((int64_t)c * S.ld + r) * 2);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float A = ((float)sh[k] + (float)sl[k]) * isa;
-                            v[k] = ((r + k == c ? J.a : 0.f) + (J.b * A + J.c * v[k])) * J.mul;
-                        }
+            fence();
+            if (J.kind == POLY) {                     // A's block, by symmetry in rows c
+#pragma unroll 4
+                for (int x = lane; x < E * E / 8; x += 64) {
+                    const int c = x / (E / 8), r = (x % (E / 8)) * 8;
+                    if (cb + c < d.m && rb + r < S.ld) {
+                        const unsigned char* q = S.hi + ((int64_t)(cb + c) * S.ld + rb + r) * 2;
+                        const uint4 h = *reinterpret_cast<const uint4*>(q), l = *reinterpret_cast<const uint4*>(q + S.step);
+                        uint2* wh = reinterpret_cast<uint2*>(mine + c * LDH + r * 2);
+                        uint2* wl = reinterpret_cast<uint2*>(lo + c * LDH + r * 2);
+                        wh[0] = make_uint2(h.x, h.y); wh[1] = make_uint2(h.z, h.w);
+                        wl[0] = make_uint2(l.x, l.y); wl[1] = make_uint2(l.z, l.w);
                     }
                 }
-                half4 h, l;
+                fence();
+            }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (r + k >= d.m || c >= nc) v[k] = 0.f;                  // the padding of both planes
-                    _Float16 hh, ll;
-                    split_pair(v[k], hh, ll);
-                    h[k] = hh; l[k] = ll;
-                }
-                if (half) {                                   // both writes, only from the triangle r >= c
+            for (int i = 0; i < E / 32; ++i)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (r + k >= c && c < d.m && r + k < D.ld) {
-                            _Float16* x = reinterpret_cast<_Float16*>(D.hi + ((int64_t)c * D.ld + r + k) * 2);
-                            x[0] = h[k];
-                            *reinterpret_cast<_Float16*>(reinterpret_cast<unsigned char*>(x) + D.step) = l[k];
-                            if (r + k < d.m) {
-                                _Float16* y = reinterpret_cast<_Float16*>(D.hi + ((int64_t)(r + k) * D.ld + c) * 2);
-                                y[0] = h[k];
-                                *reinterpret_cast<_Float16*>(reinterpret_cast<unsigned char*>(y) + D.step) = l[k];
+                for (int j = 0; j < E / 32; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x16& av = acc[bi * (E / 32) + i][bj * (E / 32) + j];
+                        const int c = j * 32 + l31, r = i * 32 + 8 * q + 4 * lh;
+                        half4* ph = reinterpret_cast<half4*>(mine + c * LDH + r * 2);
+                        half4* pl = reinterpret_cast<half4*>(lo + c * LDH + r * 2);
+                        half4 sh, sl;
+                        if (J.kind == POLY) { sh = *ph; sl = *pl; }
+                        half4 h, l;
+                        float v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            v[k] = av[4 * q + k] * mult;
+                            if (J.kind == POLY) {
+                                const float A = ((float)sh[k] + (float)sl[k]) * isa;
+                                v[k] = ((rb + r + k == cb + c ? J.a : 0.f) + (J.b * A + J.c * v[k])) * J.mul;
                             }
+                            if (rb + r + k >= d.m || cb + c >= nc) v[k] = 0.f;      // the padding of both planes
                         }
-                    continue;
-                }
-                if (c < nc && r < T.ld) {
-                    *reinterpret_cast<half4*>(T.hi + ((int64_t)c * T.ld + r) * 2) = h;
-                    *reinterpret_cast<half4*>(T.hi + T.step + ((int64_t)c * T.ld + r) * 2) = l;
-                }
-                if (c < D.ld) {
+                        split_many<4>(v, h, l);
+                        *ph = h; *pl = l;
+                    }
+            fence();
+            auto at = [&](const unsigned char* plane, int c, int r) { return *reinterpret_cast<const unsigned short*>(plane + c * LDH + r * 2); };
+            // rows c of T; a block on the diagonal takes what lies over it from the other side
+#pragma unroll 2
+            for (int x = lane; x < E * E / 8; x += 64) {
+                const int c = x / (E / 8), r = (x % (E / 8)) * 8;
+                if (cb + c >= nc || rb + r >= T.ld) continue;
+                unsigned char* o = T.hi + ((int64_t)(cb + c) * T.ld + rb + r) * 2;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (r + k < d.m) {
-                            *reinterpret_cast<_Float16*>(D.hi + ((int64_t)(r + k) * D.ld + c) * 2) = h[k];
-                            *reinterpret_cast<_Float16*>(D.hi + D.step + ((int64_t)(r + k) * D.ld + c) * 2) = l[k];
-                        }
+                for (int pl = 0; pl < 2; ++pl) {
+                    const unsigned char* src = pl ? lo : mine;
+                    const uint2 u0 = *reinterpret_cast<const uint2*>(src + c * LDH + r * 2), u1 = *reinterpret_cast<const uint2*>(src + c * LDH + r * 2 + 8);
+                    unsigned w[4] = {u0.x, u0.y, u1.x, u1.y};
+                    if (half && r < c) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (r + k < c) {
+                                const unsigned v = at(src, r + k, c);
+                                w[k / 2] = (k & 1) ? (w[k / 2] & 0xffffu) | (v << 16) : (w[k / 2] & 0xffff0000u) | v;
+                            }
+                    }
+                    *reinterpret_cast<uint4*>(o + (pl ? T.step : 0)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            if (half) continue;
+            // rows r of D
+#pragma unroll 2
+            for (int x = lane; x < E * E / 8; x += 64) {
+                const int r = x / (E / 8), c = (x % (E / 8)) * 8;
+                if (rb + r >= d.m || cb + c >= D.ld) continue;
+                unsigned char* o = D.hi + ((int64_t)(rb + r) * D.ld + cb + c) * 2;
+#pragma unroll
+                for (int pl = 0; pl < 2; ++pl) {
+                    const unsigned char* src = pl ? lo : mine;
+                    unsigned w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = at(src, c + 2 * k, r) | (unsigned)at(src, c + 2 * k + 1, r) << 16;
+                    *reinterpret_cast<uint4*>(o + (pl ? D.step : 0)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
@@ -535,7 +1070,9 @@ int64_t next_chunk(const wgs_matrix* mats, int count, const Plan& p, Cursor& c, 
         const wgs_matrix& w = mats[c.entry];
         const int left = w.batch - c.done;
         if (left <= 0) { ++c.entry; c.done = 0; continue; }
-        const int64_t one = instance_bytes(dims_of(w.rows, w.cols), p.npx, p.nt, p.ns);
+        const Dims d = dims_of(w.rows, w.cols);
+        int64_t one = instance_bytes(d, p.npx, p.nt, p.ns);
+        if (is_small(d) && small_bytes(d) > one) one = small_bytes(d);
         int64_t fit = (CHUNK_BYTES - bytes) / one;
         if (fit < 1) { if (g.count) break; fit = 1; }
         const int take = fit < left ? (int)fit : left;
@@ -559,7 +1096,12 @@ int64_t next_chunk(const wgs_matrix* mats, int count, const Plan& p, Cursor& c, 
     if (!g.count) return 0;
     int64_t sb = most / 16384;                    // 64 elements a thread where the matrix is large
     g.stat_blocks = sb < 1 ? 1 : (sb > STAT_BLOCKS ? STAT_BLOCKS : (int)sb);
-    const int64_t head = header_bytes(g.instances, g.stat_blocks);
+    g.info = up((int64_t)g.instances * g.stat_blocks * (int64_t)sizeof(Part), 256);
+    int64_t head = g.info + up((int64_t)g.instances * INFO * 4, 256);
+    g.part = 0;
+    for (int i = 0; i < g.count; ++i)
+        if (dims_of(g.mat[i].M, g.mat[i].N).np / BK > 40) g.part = head;
+    if (g.part) head += SPLIT_BYTES;
     for (int i = 0; i < g.count; ++i) g.mat[i].ws += head;
     return head + bytes;
 }
@@ -616,42 +1158,83 @@ void poly_bounds(double a, double b, double c, double top, double* q, double* ne
 }
 int ceil_log2(double v) { int e; const double f = frexp(v, &e); return f == 0.5 ? e - 1 : e; }
 
-template <int NA, int NB, int BM, int WM, int WN, int NS>
-void launch_gemm(const Group& g, const Jobs& js, int total, hipStream_t st) {
-    constexpr int sm = NS * (NA + NB) * BM * ROW;
-    auto k = ortho_gemm_kernel<NA, NB, BM, WM, WN, NS>;
+template <int NA, int NB, int BM, int WM, int WN, int NS, int E, bool SPLIT = false>
+void launch_gemm(const Group& g, const Jobs& js, int total, hipStream_t st, int most = 1, int join = 0) {
+    constexpr int stages = NS * (NA + NB) * BM * ROW, blocks = WM * WN * E * (E + 4) * 4;
+    constexpr int sm = stages > blocks ? stages : blocks;
+    static_assert(sm <= 160 * 1024, "LDS of a CU");
+    auto k = ortho_gemm_kernel<NA, NB, BM, WM, WN, NS, E, SPLIT>;
     (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
-    WGS_LAUNCH(k, dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN), sm, st, g, js, total);
+    const int per = (total + 7) / 8, run = (per + (per + 31) / 32 - 1) / ((per + 31) / 32);
+    WGS_LAUNCH(k, dim3((unsigned)((per + run - 1) / run * run * 8)), dim3(64 * WM * WN), sm, st, js, total, run, most, join, g);
 }
-int tiles_of(const Group& g, const Jobs& js, int bm) {
+int tiles_of(const Group& g, const Jobs& js, int bm, int most = 1) {
     int64_t t = 0;
     for (int i = 0; i < g.count; ++i) {
         const Dims d = dims_of(g.mat[i].M, g.mat[i].N);
         const int64_t tm = (d.m + bm - 1) / bm, tn = (d.n + bm - 1) / bm;
-        t += g.mat[i].batch * (js.sym ? tm * (tm + 1) / 2 : tm * tn);
+        t += g.mat[i].batch * (js.sym ? tm * (tm + 1) / 2 : tm * tn) * parts_of_sum((js.kgram ? d.np : d.mp) / BK, most);
     }
     t *= js.count;
     return t < (1LL << 30) ? (int)t : 0;
 }
 template <int NA, int NB>
 int gemm(const Group& g, const Jobs& js, hipStream_t st) {
+    // Tile side.  Cost of a choice: rounds of tiles over the CUs (two workgroups a CU up to 128) times a tile's area; half of it by the mean,
+    // since CUs that a last round leaves idle let the others clock higher (the products run at the card's power limit).
     int bm = 64;
-    if (tiles_of(g, js, 256) >= 200) bm = 256;
-    else if (tiles_of(g, js, 128) >= 200) bm = 128;
+    double best = 1e300;
+    for (int s : {64, 128, 192, 256}) {
+        const int t = tiles_of(g, js, s);
+        if (t <= 0) continue;
+        const double slots = s <= 128 ? 512 : 256, rounds = 0.5 * (ceil(t / slots) + t / slots);
+        const double cost = rounds * s * s * (s == 64 ? 2 * 1.6 : s == 128 ? 2 * 1.1 : 1.0);
+        if (cost < best) { best = cost; bm = s; }
+    }
     const int total = tiles_of(g, js, bm);
     WGS_CHECK_ARG(total > 0, "orthogonalise: too many matrices for one launch");
-    if (bm == 256) launch_gemm<NA, NB, 256, 2, 4, 2>(g, js, total, st);
-    else if (bm == 128) launch_gemm<NA, NB, 128, 2, 2, 2>(g, js, total, st);
-    else launch_gemm<NA, NB, 64, 2, 2, 4>(g, js, total, st);
+    if (bm == 256) launch_gemm<NA, NB, 256, 2, 4, 2, 64>(g, js, total, st);
+    else if (bm == 192) launch_gemm<NA, NB, 192, 2, 2, 3, 96>(g, js, total, st);
+    else if (bm == 128) launch_gemm<NA, NB, 128, 2, 2, 2, 64>(g, js, total, st);
+    else if (total <= 256) {
+        // Parts where the tiles leave half the CUs idle, up to three workgroups a CU, and where they save over 40 chunks (some 0.24 us each) of the
+        // longest sum for a second launch of some 8 us (512 x 4608 fp32: 403 -> 303 us; with 136 and 216 tiles: 402 -> 438, 738 -> 827).
+        int most = 1, longest = 0;
+        for (int i = 0; i < g.count; ++i) {
+            const Dims d = dims_of(g.mat[i].M, g.mat[i].N);
+            const int nk = (js.kgram ? d.np : d.mp) / BK;
+            if (nk > longest) longest = nk;
+        }
+        if (g.part && js.count == 1 && total <= 128)
+            for (int x = 2; x <= 16 && tiles_of(g, js, 64, x) <= 768; ++x) most = x;
+        if (longest - longest / parts_of_sum(longest, most) > 40) {
+            launch_gemm<NA, NB, 64, 2, 2, 4, 32, true>(g, js, tiles_of(g, js, 64, most), st, most);
+            launch_gemm<NA, NB, 64, 2, 2, 4, 32, true>(g, js, total, st, most, 1);
+        } else launch_gemm<NA, NB, 64, 2, 2, 8, 32>(g, js, total, st);
+    }
+    else launch_gemm<NA, NB, 64, 2, 2, 4, 32>(g, js, total, st);
     return WGS_OK;
 }
 
 template <int DT, bool STEP>
 void launch_prepare(const Group& g, const Momentum& mo, const Bounds& bd, hipStream_t st) {
-    WGS_LAUNCH((ortho_norm_kernel<DT, STEP>), dim3((unsigned)(g.instances * g.stat_blocks)), dim3(256), 0, st, g, mo);
+    WGS_LAUNCH((ortho_norm_kernel<DT, STEP>), dim3((unsigned)(g.instances * g.stat_blocks)), dim3(512), 0, st, g, mo);
     int64_t tiles = 0;
     for (int i = 0; i < g.count; ++i) tiles += (int64_t)g.mat[i].batch * ((up(g.mat[i].M, BK) + 63) / 64) * ((up(g.mat[i].N, BK) + 63) / 64);
     WGS_LAUNCH((ortho_split_kernel<DT, STEP>), dim3((unsigned)tiles), dim3(256), 0, st, g, mo, bd, (int)tiles);
+}
+
+bool all_small(const Group& g) {
+    for (int i = 0; i < g.count; ++i)
+        if (!is_small(dims_of(g.mat[i].M, g.mat[i].N))) return false;
+    return true;
+}
+void launch_small(const Group& g, const Momentum& mo, const SmallArgs& ar, hipStream_t st) {
+    int m = 0;
+    for (int i = 0; i < g.count; ++i) { const int x = dims_of(g.mat[i].M, g.mat[i].N).m; if (x > m) m = x; }
+    const dim3 gr((unsigned)g.instances), bl(64 * SMALL_WAVES);
+    if (m <= 32) WGS_LAUNCH(ortho_small_kernel<1>, gr, bl, 0, st, g, mo, ar);
+    else WGS_LAUNCH(ortho_small_kernel<2>, gr, bl, 0, st, g, mo, ar);
 }
 
 int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step, const Momentum& mo, int steps, double a, double b, double c, float eps, void* ws,
@@ -678,7 +1261,14 @@ int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step
     Cursor cur;
     Group g;
     g.dtype = dtype; g.step = step; g.npx = p.npx; g.nt = p.nt; g.ns = p.ns; g.ws = (unsigned char*)ws;
+    SmallArgs sm;
+    sm.bd = bd; sm.a = (float)a; sm.b = (float)b; sm.c = (float)c;
+    for (int t = 0; t < steps; ++t) sm.sb[t] = (float)ldexp(1.0, 14 - ceil_log2(q[t]));
     while (next_chunk(mats, count, p, cur, g) > 0) {
+        if (all_small(g)) {
+            launch_small(g, mo, sm, st);
+            continue;
+        }
         if (step) {
             if (dtype == WGS_F32) launch_prepare<WGS_F32, true>(g, mo, bd, st);
             else if (dtype == WGS_BF16) launch_prepare<WGS_BF16, true>(g, mo, bd, st);
@@ -701,10 +1291,11 @@ int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step
                 j.kind = kind; j.p = op; j.r = orr; j.dst = dst; j.t = t; j.first = ph == 0; j.mul = 1.f;
                 return j;
             };
-            js.count = 1; js.sym = 1;
+            js.count = 1; js.sym = 1; js.kgram = 1;
             job(0, GRAM, BUF_X, BUF_X, A);
             rc = single ? gemm<1, 1>(g, js, st) : gemm<2, 2>(g, js, st);
             if (rc) return rc;
+            js.kgram = 0;
             double sq = 1.0;
             for (int it = 0; it < p.len[ph]; ++it, ++t) {
                 const int em = ceil_log2(q[t]);
