@@ -61,13 +61,19 @@ def parse(argv=None):
     ext.add_argument('--check-precision', type=int, default=0, metavar='N',
                      help="every N iterations regenerate the batch's images with the exact-fp32 kernels and report / check the "
                           "16-bit mode's image error against the 1e-3 gate (0 = off)")
+    ext.add_argument('--optimizer', choices=('adam', 'muon'), default='adam',
+                     help="update of the reconstructor's convolution weights: adam = the reference's; muon = orthogonalised momentum, steps of "
+                          "the size of Adam's at --reconstructor-lr (all other parameters: Adam)")
+    ext.add_argument('--lambda-ent', type=float, default=0.0, help="weight of the mean entropy of the path scores, subtracted from the loss")
+    ext.add_argument('--label-top', type=int, default=0, metavar='K', help="report the accuracy of the K most likely paths too (0 = off)")
     return p.parse_args(argv)
 
 
 def main(argv=None):
     args = parse(argv)
     ext = {'random_init_generator': args.random_init_generator, 'seed': args.seed, 'precision': args.precision,
-           'r_precision': args.r_precision, 'check_precision': args.check_precision}
+           'r_precision': args.r_precision, 'check_precision': args.check_precision, 'optimizer': args.optimizer,
+           'lambda_ent': args.lambda_ent, 'label_top': args.label_top}
     for k in ext:
         delattr(args, k)
     world = int(os.environ.get('WORLD_SIZE', '1'))
@@ -110,6 +116,7 @@ def main(argv=None):
     args.precision = ext['precision'] or C.DEFAULT_PRECISION
     args.r_precision = ext['r_precision']
     args.check_precision = ext['check_precision']
+    args.optimizer, args.lambda_ent, args.label_top = ext['optimizer'], ext['lambda_ent'], ext['label_top']
     trn = Trainer(params=args, exp_dir=exp_dir, use_cuda=use_cuda, multi_gpu=world > 1)
     trn.train(generator=G, support_sets=S, reconstructor=R)
     if world > 1:

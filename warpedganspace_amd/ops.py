@@ -309,57 +309,96 @@ def _matrix_view(t):
     return None
 
 
-@torch.no_grad()
+class MuonUpdate:
+    """The step of `muon_step` on tensors that stay where they are: checked and described once, then `step(lr)` any number of times.
+
+    It keeps the tensors themselves (and so their memory), not results: every call reads the gradients and updates momenta and weights in place,
+    on the current stream of their device; its workspace comes from torch's allocator, call by call."""
+
+    def __init__(self, params, grads, momenta, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, grad_scale=1.0, steps=5,
+                 coefficients=NS_COEFFICIENTS, eps=1e-7):
+        if not (len(params) == len(grads) == len(momenta)):
+            raise L.WgsError("muon_step: %d params, %d grads, %d momenta" % (len(params), len(grads), len(momenta)))
+        if not 0.0 <= momentum < 1.0:
+            raise L.WgsError("momentum must be in [0, 1), got %s" % (momentum,))
+        if not 1 <= int(steps) <= 16:
+            raise L.WgsError("steps must be 1 .. 16, got %s" % (steps,))
+        if isinstance(scale, str) and scale != 'rms':
+            raise L.WgsError("scale must be None, a number or 'rms', got %r" % (scale,))
+        self.tensors = (list(params), list(grads), list(momenta))
+        self.weight_decay, self.grad_scale, self.steps = weight_decay, grad_scale, int(steps)
+        self.args = (L.c_float(momentum), int(bool(nesterov)))
+        self.rest = tuple(L.c_float(v) for v in coefficients) + (L.c_float(eps),)
+        self.n = len(params)
+        if not self.n:
+            return
+        self.device, self.dtype = dev, dtype = params[0].device, params[0].dtype
+        self.mats = ctypes.create_string_buffer(_MATRIX.size * self.n)
+        self.factors, spans = [], []
+        for k, (w, g, m) in enumerate(zip(params, grads, momenta)):
+            _check_matrix(w, 'param', dev, dtype)
+            _check_matrix(g, 'grad', dev, dtype)
+            if m.dtype != torch.float32 or m.device != dev or m.shape != w.shape or g.shape != w.shape:
+                raise L.WgsError("a momentum must be float32 of its param's shape on its device, got %s %s on %s and grad %s for param %s" % (
+                    m.dtype, tuple(m.shape), m.device, tuple(g.shape), tuple(w.shape)))
+            if w.dim() != 2 and not (w.stride() == m.stride() == g.stride()):
+                raise L.WgsError("a convolution weight, its gradient and its momentum must have the same layout, got strides %s %s %s" % (
+                    w.stride(), g.stride(), m.stride()))
+            w2, g2, m2 = _matrix_view(w), _matrix_view(g), _matrix_view(m)
+            if w2 is None or g2 is None or m2 is None:
+                raise L.WgsError("muon_step takes matrices and dense convolution weights, got shape %s strides %s" % (tuple(w.shape), w.stride()))
+            M, N = w2.shape
+            if not m2.is_contiguous():
+                raise L.WgsError("momentum must be contiguous")
+            for t, what in ((w2, 'param'), (g2, 'grad')):
+                if (N > 1 and t.stride(1) != 1) or (M > 1 and t.stride(0) < N):
+                    raise L.WgsError("%s: the elements of a row must be adjacent, got strides %s" % (what, t.stride()))
+            gr, wr = (g2.stride(0), w2.stride(0)) if M > 1 else (N, N)
+            spans.append((m2.data_ptr(), m2.data_ptr() + 4 * M * N, True))
+            spans.append((w2.data_ptr(), w2.data_ptr() + w2.element_size() * ((M - 1) * wr + N), wr == N))
+            self.factors.append(max(1.0, M / N) ** 0.5 if scale is None else 0.2 * max(M, N) ** 0.5 if scale == 'rms' else float(scale))
+            _MATRIX.pack_into(self.mats, k * _MATRIX.size, g2.data_ptr(), w2.data_ptr(), m2.data_ptr(), 0, 0, gr, wr, M, N, 1, 0.0, 1.0, 0)
+        _check_apart(spans)
+        self.code = _DTYPES[dtype]
+        self.need = L.lib().wgs_muon_step_ws_bytes(self.mats, self.n, self.code, self.steps)
+        self.lr = None
+
+    @torch.no_grad()
+    def step(self, lr):
+        if not self.n:
+            return
+        if lr != self.lr:
+            decay = 1.0 - lr * self.weight_decay
+            for k, f in enumerate(self.factors):
+                _STEP_DECAY.pack_into(self.mats, k * _MATRIX.size + _STEP_DECAY_AT, lr * f, decay)
+            self.lr = lr
+        with _on(self.device):
+            ws = torch.empty(self.need, dtype=torch.uint8, device=self.device)
+            L.check(L.lib().wgs_muon_step(self.mats, self.n, self.code, self.args[0], self.args[1], L.c_float(self.grad_scale), self.steps, *self.rest,
+                                          L.rawptr(ws), L.c_int64(self.need), L.stream()), 'wgs_muon_step')
+
+
+_STEP_DECAY, _STEP_DECAY_AT = struct.Struct('=2f'), struct.calcsize('=3Q4q3i')
+
+
+def _check_apart(spans):
+    """What a step writes may not overlap: spans (start, end, dense) in bytes.  A span that begins inside a dense one overlaps it; inside a strided
+    one it may lie between the rows."""
+    spans = sorted(spans)
+    for (a0, a1, dense), (b0, _, _) in zip(spans, spans[1:]):
+        if b0 == a0 or (dense and b0 < a1):
+            raise L.WgsError("muon_step: a param or momentum is given twice, or overlaps another")
+
+
 def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, grad_scale=1.0, steps=5,
               coefficients=NS_COEFFICIENTS, eps=1e-7):
-    """One update of many matrices in place, in the launches of one:
+    """One update of many matrices in place, in the launches of one (instead of torch.optim.Adam's, lib/trainer.py:153-156, for these weights):
 
         momentum buffer  m <- momentum m + g,        u = g + momentum m (nesterov) or m       (g = grad_scale * gradient)
-        weight           W <- (1 - lr weight_decay) W - lr f O,   O = orthogonalise(u),   f = sqrt(max(1, M / N)), or `scale` where given
+        weight           W <- (1 - lr weight_decay) W - lr f O,   O = orthogonalise(u)
+        f = sqrt(max(1, M / N)) where scale is None, 0.2 sqrt(max(M, N)) for 'rms' (steps of the size of Adam's), or the number given
 
     params, grads: matrices [M, N] (rows may be strided, elements of a row adjacent), or convolution weights [Co, Ci, kh, kw], contiguous or
     channels-last, taken as [Co, Ci kh kw]; float32, bfloat16 or float16, one type a call.  momenta: float32 of the same shape and order,
-    contiguous.  The stored momentum and the whole update are fp32; weights are rounded once."""
-    if not (len(params) == len(grads) == len(momenta)):
-        raise L.WgsError("muon_step: %d params, %d grads, %d momenta" % (len(params), len(grads), len(momenta)))
-    if not params:
-        return
-    if not 0.0 <= momentum < 1.0:
-        raise L.WgsError("momentum must be in [0, 1), got %s" % (momentum,))
-    if not 1 <= int(steps) <= 16:
-        raise L.WgsError("steps must be 1 .. 16, got %s" % (steps,))
-    dev, dtype = params[0].device, params[0].dtype
-    entries, seen = [], set()
-    decay = 1.0 - lr * weight_decay
-    for w, g, m in zip(params, grads, momenta):
-        _check_matrix(w, 'param', dev, dtype)
-        _check_matrix(g, 'grad', dev, dtype)
-        if m.dtype != torch.float32 or m.device != dev or m.shape != w.shape or g.shape != w.shape:
-            raise L.WgsError("a momentum must be float32 of its param's shape on its device, got %s %s on %s and grad %s for param %s" % (
-                m.dtype, tuple(m.shape), m.device, tuple(g.shape), tuple(w.shape)))
-        if w.dim() != 2 and not (w.stride() == m.stride() == g.stride()):
-            raise L.WgsError("a convolution weight, its gradient and its momentum must have the same layout, got strides %s %s %s" % (
-                w.stride(), g.stride(), m.stride()))
-        w2, g2, m2 = _matrix_view(w), _matrix_view(g), _matrix_view(m)
-        if w2 is None or g2 is None or m2 is None:
-            raise L.WgsError("muon_step takes matrices and dense convolution weights, got shape %s strides %s" % (tuple(w.shape), w.stride()))
-        M, N = w2.shape
-        if not m2.is_contiguous():
-            raise L.WgsError("momentum must be contiguous")
-        for t, what in ((w2, 'param'), (g2, 'grad')):
-            if (N > 1 and t.stride(1) != 1) or (M > 1 and t.stride(0) < N):
-                raise L.WgsError("%s: the elements of a row must be adjacent, got strides %s" % (what, t.stride()))
-        if w2.data_ptr() in seen or m2.data_ptr() in seen:
-            raise L.WgsError("muon_step: a param or momentum is given twice")
-        seen.add(w2.data_ptr())
-        seen.add(m2.data_ptr())
-        f = max(1.0, M / N) ** 0.5 if scale is None else scale
-        gr, wr = (g2.stride(0), w2.stride(0)) if M > 1 else (N, N)
-        entries.append((g2.data_ptr(), w2.data_ptr(), m2.data_ptr(), 0, 0, gr, wr, M, N, 1, lr * f, decay, 0))
-    lib = L.lib()
-    a, b, c = (L.c_float(v) for v in coefficients)
-
-    def call(mats, n, code, ws, need):
-        L.check(lib.wgs_muon_step(mats, n, code, L.c_float(momentum), int(bool(nesterov)), L.c_float(grad_scale), int(steps), a, b, c, L.c_float(eps),
-                                  ws, need, L.stream()), 'wgs_muon_step')
-    _run_matrices(entries, lib.wgs_muon_step_ws_bytes, call, dtype, dev, int(steps))
+    contiguous.  What is written may not overlap.  The stored momentum and the whole update are fp32; weights are rounded once."""
+    MuonUpdate(params, grads, momenta, momentum, nesterov, weight_decay, scale, grad_scale, steps, coefficients, eps).step(lr)

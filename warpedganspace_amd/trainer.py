@@ -29,6 +29,7 @@ import torch.distributed as dist
 
 from . import _lib as L
 from . import conv as C
+from . import ops
 from .aux import TrainingStatTracker, sample_z, sec2dhms, update_progress, update_stdout
 from .support_sets import rbf_workspace
 
@@ -82,16 +83,22 @@ class FlatBucket:
     and Adam moment buffers.  `gview[id(p)]` is the gradient region of p in p's MEMORY layout (conv weights:
     packed [Co, kh*kw, Ci])."""
 
-    def __init__(self, groups, device):
-        # groups: list of (lr, [params])
+    def __init__(self, groups, device, muon=False):
+        # groups: list of (lr, [params]).  muon: the convolution weights of the first group come first in it and are updated by ops.muon_step
+        # (their momenta live where Adam's first moments would), everything else by Adam.
         self.segments, self.gview, self.groups = [], {}, []
+        self.muon_end, self._muon = 0, None
         total = 0
-        for lr, params in groups:
+        for gi, (lr, params) in enumerate(groups):
             start = total
+            if muon and gi == 0:
+                params = [p for p in params if p.dim() == 4] + [p for p in params if p.dim() != 4]
             for p in params:
                 n = (p.numel() + 3) & ~3
                 self.segments.append((p, total, p.numel()))
                 total += n
+                if muon and gi == 0 and p.dim() == 4:
+                    self.muon_end = total
             self.groups.append((lr, start, total))
         self.flat = torch.zeros(total, device=device)
         self.grad = torch.zeros(total, device=device)
@@ -116,9 +123,21 @@ class FlatBucket:
     def zero_grad(self):
         self.grad.zero_()
 
+    def muon_step(self, world=1):
+        """The first group's convolution weights, as [Co, kh kw Ci] matrices: momentum, orthogonalisation, update; steps of Adam's size ('rms')."""
+        if self._muon is None:
+            views = []
+            for buf in (self.flat, self.grad, self.exp_avg):
+                views.append([buf[off:off + n].view(p.shape[0], -1) for p, off, n in self.segments if off < self.muon_end])
+            self._muon = ops.MuonUpdate(*views, scale='rms', grad_scale=1.0 / world)
+        self._muon.step(self.groups[0][0])
+
     def adam_step(self, world=1, betas=(0.9, 0.999), eps=1e-8):
         self.step_count += 1
+        if self.muon_end:
+            self.muon_step(world)
         for lr, a, b in self.groups:
+            a = max(a, self.muon_end)
             if b > a:
                 L.check(L.lib().wgs_adam_step(L.rawptr(self.flat[a:]), L.rawptr(self.grad[a:]), L.rawptr(self.exp_avg[a:]),
                                               L.rawptr(self.exp_avg_sq[a:]), L.c_int64(b - a), L.c_float(lr),
@@ -180,7 +199,14 @@ class TrainStep:
         r_params = [p for n, p in reconstructor.named_parameters()
                     if p.requires_grad and not n.startswith('features_extractor.fc')]
         s_params = [p for p in support_sets.parameters() if p.requires_grad]
-        self.bucket = FlatBucket([(params.reconstructor_lr, r_params), (params.support_set_lr, s_params)], device)
+        # extensions of the objective and the optimiser (all off by default: the reference's step)
+        self.optimizer = getattr(params, 'optimizer', None) or 'adam'
+        if self.optimizer not in ('adam', 'muon'):
+            raise ValueError("optimizer must be 'adam' or 'muon', got %r" % (self.optimizer,))
+        self.lambda_ent = float(getattr(params, 'lambda_ent', 0.0) or 0.0)      # total loss -= lambda_ent * mean entropy of the path scores
+        self.label_top = min(int(getattr(params, 'label_top', 0) or 0), support_sets.ALPHAS.shape[0], ops.TOP_MAX)      # top-k accuracy statistic
+        self.extra_sum = torch.zeros(2, device=device)                          # (mean entropy, top-k accuracy) since the last pop_stats
+        self.bucket = FlatBucket([(params.reconstructor_lr, r_params), (params.support_set_lr, s_params)], device, muon=self.optimizer == 'muon')
         if world > 1:
             # replicas start from rank 0's parameters and BN running statistics, whatever each rank's RNG produced
             dist.broadcast(self.bucket.flat, 0)
@@ -215,12 +241,12 @@ class TrainStep:
     # -- optimizer state (optional 'optim' key of checkpoint.pt; reference readers ignore unknown keys) ---------
     def optim_state(self):
         b = self.bucket
-        return {'step': b.step_count, 'exp_avg': b.exp_avg.detach().cpu().clone(), 'exp_avg_sq': b.exp_avg_sq.detach().cpu().clone(),
+        return {'optimizer': self.optimizer, 'step': b.step_count, 'exp_avg': b.exp_avg.detach().cpu().clone(), 'exp_avg_sq': b.exp_avg_sq.detach().cpu().clone(),
                 'layout': [(n, off) for (_, off, n) in b.segments]}
 
     def load_optim_state(self, st):
         b = self.bucket
-        if st is None or st.get('layout') != [(n, off) for (_, off, n) in b.segments]:
+        if st is None or st.get('optimizer', 'adam') != self.optimizer or st.get('layout') != [(n, off) for (_, off, n) in b.segments]:
             return False
         b.step_count = int(st['step'])
         b.exp_avg.copy_(st['exp_avg'].to(b.exp_avg.device))
@@ -536,6 +562,8 @@ class TrainStep:
                                    L.c_float(p.lambda_cls), L.c_float(p.lambda_reg), L.ptr(self.dlogits), L.ptr(self.dmag),
                                    L.ptr(self.stats), L.ptr(self.argmax, torch.int64), L.ptr(self.loss_ws), B, self.K, st),
                 'wgs_ce_l1_loss')                                             # :245-249,257-258
+        if self.lambda_ent or self.label_top:
+            self._label_terms(logits, idx)
         gb = self.bucket.gview
         # R's conv weight gradients are not needed for d_img: they are queued and run on the side stream, next to the
         # generator's backward (whose 4x4..32x32 layers under-fill the chip); the ResNet path only (LeNet computes them inline)
@@ -615,6 +643,20 @@ class TrainStep:
         self.steps_done += 1
         return self.stats
 
+    def _label_terms(self, logits, idx):
+        """The entropy term of the loss (its gradient is added to dlogits, its value to the total loss) and the top-k accuracy."""
+        lg = logits.detach().requires_grad_(self.lambda_ent != 0.0)
+        with torch.enable_grad():
+            r = ops.label_logprobs(lg, idx, top=self.label_top)
+        ent = r.entropy.detach().mean()
+        if self.lambda_ent:
+            d, = torch.autograd.grad(r.entropy, lg, torch.full_like(r.entropy, -self.lambda_ent / self.B))
+            self.dlogits += d
+            self.stats[2] -= self.lambda_ent * ent
+        self.extra_sum[0] += ent
+        if self.label_top:
+            self.extra_sum[1] += (r.top_index == idx[:, None]).any(1).float().mean()
+
     def pop_stats(self):
         """Mean (accuracy, classification_loss, regression_loss, total_loss) since the last call (one sync)."""
         s = self.stats_sum.clone()
@@ -622,9 +664,20 @@ class TrainStep:
             dist.all_reduce(s)
             s /= self.world
         v = (s / max(self.stats_n, 1)).tolist()
+        out = {'accuracy': v[3], 'classification_loss': v[0], 'regression_loss': v[1], 'total_loss': v[2]}
+        if self.lambda_ent or self.label_top:
+            e = self.extra_sum.clone()
+            if self.world > 1:
+                dist.all_reduce(e)
+                e /= self.world
+            e = (e / max(self.stats_n, 1)).tolist()
+            out['entropy'] = e[0]
+            if self.label_top:
+                out['top%d_accuracy' % self.label_top] = e[1]
+            self.extra_sum.zero_()
         self.stats_sum.zero_()
         self.stats_n = 0
-        return {'accuracy': v[3], 'classification_loss': v[0], 'regression_loss': v[1], 'total_loss': v[2]}
+        return out
 
 
 class Trainer(object):
