@@ -76,14 +76,18 @@ __host__ __device__ __forceinline__ int64_t instance_bytes(const Dims& d, int np
 }
 // Buffers of an instance: 0 = X, 1 / 2 = X^T (the second one where a phase's result is another phase's input), 3.. = m x m
 enum { BUF_X = 0, BUF_T0 = 1, BUF_T1 = 2, BUF_S = 3 };
-struct Plane { unsigned char* hi; int64_t step; int ld; int64_t bytes; };       // lo plane = hi + step
-__device__ __forceinline__ Plane plane_of(const Group& g, const Mat& a, const Dims& d, int inst, int buf) {
+// A matrix of pairs keeps, row by row, 32 hi parts and their 32 lo parts in turn: one cache line holds what a row gives a chunk of the sum.  (As two
+// planes, 64 bytes of a row each, the loads fetch half lines: measured half the rate into the LDS.)  A matrix of hi parts alone is plain.
+struct Plane { unsigned char* p; int ld, pair; };
+__device__ __forceinline__ int row_bytes(const Plane& q) { return q.ld * (q.pair ? 4 : 2); }
+__device__ __forceinline__ unsigned char* at_hi(const Plane& q, int r, int k) {      // the lo part: 64 bytes on
+    return q.p + (int64_t)r * row_bytes(q) + (q.pair ? (k >> 5) * 128 + (k & 31) * 2 : k * 2);
+}
+__device__ __forceinline__ Plane plane_of(const Group& g, const Mat& a, const Dims& d, int inst, int buf, bool pair = true) {
     unsigned char* p = g.ws + a.ws + inst * instance_bytes(d, g.npx, g.nt, g.ns);
-    Plane r;
-    if (buf == BUF_X) { r = Plane{p, d.szx, d.np, (int64_t)d.m * d.np * 2}; }
-    else if (buf < BUF_S) { r = Plane{p + g.npx * d.szx + (int64_t)(buf - 1) * g.npx * d.szt, d.szt, d.mp, (int64_t)d.n * d.mp * 2}; }
-    else { r = Plane{p + g.npx * d.szx + (int64_t)g.nt * g.npx * d.szt + (int64_t)(buf - BUF_S) * 2 * d.szs, d.szs, d.mp, (int64_t)d.m * d.mp * 2}; }
-    return r;
+    if (buf == BUF_X) return Plane{p, d.np, pair};
+    if (buf < BUF_S) return Plane{p + g.npx * d.szx + (int64_t)(buf - 1) * g.npx * d.szt, d.mp, pair};
+    return Plane{p + g.npx * d.szx + (int64_t)g.nt * g.npx * d.szt + (int64_t)(buf - BUF_S) * 2 * d.szs, d.mp, 1};
 }
 // header of the workspace: partial norms, then the scalars of every instance
 struct Part { double ss; float amax; float pad; };
@@ -328,15 +332,15 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(const Group g, const M
     }
     __syncthreads();
     const bool wide = a.M <= a.N;
-    const Plane nat = plane_of(g, a, d, b, wide ? BUF_X : BUF_T0), tra = plane_of(g, a, d, b, wide ? BUF_T0 : BUF_X);
+    const Plane nat = plane_of(g, a, d, b, wide ? BUF_X : BUF_T0, LO), tra = plane_of(g, a, d, b, wide ? BUF_T0 : BUF_X, LO);
     // natural: rows r < M, columns up to the padding; transposed: rows c < N, columns r up to the padding.  Eight columns (16 bytes) a thread;
     // the padded lengths are multiples of 32.
     auto put = [&](const Plane& p, int row, int col, const float (&v)[8]) {
         half8 h, l;
         split_many<8>(v, h, l);
-        unsigned char* q = p.hi + ((int64_t)row * p.ld + col) * 2;
+        unsigned char* q = at_hi(p, row, col);
         *reinterpret_cast<half8*>(q) = h;
-        if (LO) *reinterpret_cast<half8*>(q + p.step) = l;
+        if (LO) *reinterpret_cast<half8*>(q + 64) = l;
     };
 #pragma unroll
     for (int i = t; i < 64 * 8; i += 256) {
@@ -699,9 +703,9 @@ __device__ __forceinline__ void tile_lower(int t, int tm, int& ti, int& tj) {
 template <int NA, int NB, int BM, int WAVES_M, int WAVES_N, int NS, int E, bool SPLIT = false>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(const Jobs js, int total, int run, int most, int join, const Group g) {
     constexpr int BN = BM, NW = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 32, TN = WN / 32;
-    constexpr int A_BYTES = BM * ROW, B_BYTES = BN * ROW, STAGE = NA * A_BYTES + NB * B_BYTES;
-    constexpr int AI = BM / 16 / NW, BI = BN / 16 / NW, NPIECE = NA * AI + NB * BI;
-    static_assert(AI * 16 * NW == BM && BI * 16 * NW == BN && TM * 32 * WAVES_M == BM && TN * 32 * WAVES_N == BN, "tile / wave count mismatch");
+    constexpr int RA = NA * ROW, RB = NB * ROW, A_BYTES = BM * RA, B_BYTES = BN * RB, STAGE = A_BYTES + B_BYTES;      // bytes of a row, an operand, a chunk
+    constexpr int GA = 1024 / RA, GB = 1024 / RB, AI = BM / GA / NW, BI = BN / GB / NW, NPIECE = AI + BI;               // rows of a load, loads of a wave
+    static_assert(AI * GA * NW == BM && BI * GB * NW == BN && TM * 32 * WAVES_M == BM && TN * 32 * WAVES_N == BN, "tile / wave count mismatch");
     static_assert(WM % E == 0 && WN % E == 0, "epilogue block");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -740,41 +744,37 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
     if (js.sym) tile_lower(tile % per, tm, ti, tj);
     else tile_full(tile % per, tm, tn, ti, tj);
     const int i0 = ti * BM, j0 = tj * BN;
-    const Plane P = plane_of(g, mat, d, b, J.p), R = plane_of(g, mat, d, b, J.r);
+    const Plane P = plane_of(g, mat, d, b, J.p, NA == 2), R = plane_of(g, mat, d, b, J.r, NB == 2);
     const int nk_all = P.ld / BK, k0 = SPLIT ? nk_all * part / parts : 0, nk = SPLIT ? nk_all * (part + 1) / parts - k0 : nk_all;
-
-    const __amdgpu_buffer_rsrc_t rp0 = __builtin_amdgcn_make_buffer_rsrc(P.hi, 0, (unsigned)P.bytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rp1 = __builtin_amdgcn_make_buffer_rsrc(P.hi + (NA > 1 ? P.step : 0), 0, (unsigned)P.bytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rr0 = __builtin_amdgcn_make_buffer_rsrc(R.hi, 0, (unsigned)R.bytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rr1 = __builtin_amdgcn_make_buffer_rsrc(R.hi + (NB > 1 ? R.step : 0), 0, (unsigned)R.bytes, 0x00020000);
-    // An LDS load writes wave base + lane * 16: one instruction fills 16 rows of 64 bytes.  The four 16-byte slots of a row are permuted by
-    // (row >> 2) & 3, on the address that is fetched and on the one that is read, so that the rows of a fragment read spread over the banks.
-    const int lrow = lane >> 2, slot = lane & 3;
+    const int rows_r = J.kind >= APPLY_MID ? d.n : d.m;
+    const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc(P.p, 0, (unsigned)(d.m * row_bytes(P)), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rr = __builtin_amdgcn_make_buffer_rsrc(R.p, 0, (unsigned)(rows_r * row_bytes(R)), 0x00020000);
+    // An LDS load writes wave base + lane * 16: one instruction fills 8 rows of 128 bytes (32 hi, 32 lo) or 16 of 64.  The 16-byte slots of a row
+    // are permuted by the row's number, on the address that is fetched and on the one that is read, so that the rows of a fragment read spread
+    // over all banks.
+    auto twist = [](int row, int n) { return n == 2 ? (row >> 1) & 7 : (row >> 2) & 3; };
     int a_off[AI], b_off[BI];
 #pragma unroll
     for (int j = 0; j < AI; ++j) {
-        const int row = (wave * AI + j) * 16 + lrow, lc = slot ^ ((row >> 2) & 3);
-        a_off[j] = i0 + row < d.m ? (int)(((int64_t)(i0 + row) * P.ld + lc * 8) * 2) : OOB;
+        const int row = (wave * AI + j) * GA + lane / (64 / GA), lc = lane % (64 / GA) ^ twist(row, NA);
+        a_off[j] = i0 + row < d.m ? (i0 + row) * row_bytes(P) + lc * 16 : OOB;
     }
-    const int rows_r = J.kind >= APPLY_MID ? d.n : d.m;
 #pragma unroll
     for (int j = 0; j < BI; ++j) {
-        const int row = (wave * BI + j) * 16 + lrow, lc = slot ^ ((row >> 2) & 3);
-        b_off[j] = j0 + row < rows_r ? (int)(((int64_t)(j0 + row) * R.ld + lc * 8) * 2) : OOB;
+        const int row = (wave * BI + j) * GB + lane / (64 / GB), lc = lane % (64 / GB) ^ twist(row, NB);
+        b_off[j] = j0 + row < rows_r ? (j0 + row) * row_bytes(R) + lc * 16 : OOB;
     }
     // piece x of the next chunk (chunk nC, behind the last one that one again: its data is not used) into stage buf
     int nC = 0;
     auto piece = [&](int buf, int x) {
-        const int adv = (k0 + (nC < nk ? nC : nk - 1)) * ROW;
+        const int c = k0 + (nC < nk ? nC : nk - 1);
         lds_byte* st = (lds_byte*)(smem + buf * STAGE);
-        if (x < NA * AI) {
-            const int j = x / NA, pl = x % NA;
-            const int off = a_off[j];
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(pl ? rp1 : rp0, st + (wave * AI + j) * 16 * ROW + pl * A_BYTES, 16, off, adv, 0, 0);
+        if (x < AI) {
+            const int off = a_off[x];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, st + (wave * AI + x) * 1024, 16, off, c * RA, 0, 0);
         } else {
-            const int j = (x - NA * AI) / NB, pl = (x - NA * AI) % NB;
-            const int off = b_off[j];
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(pl ? rr1 : rr0, st + NA * A_BYTES + (wave * BI + j) * 16 * ROW + pl * B_BYTES, 16, off, adv, 0, 0);
+            const int off = b_off[x - AI];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, st + A_BYTES + (wave * BI + x - AI) * 1024, 16, off, c * RB, 0, 0);
         }
     };
 
@@ -785,14 +785,14 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    const int l31 = lane & 31, lh = lane >> 5, swz = (l31 >> 2) & 3;
-    const int a_rd = (wm * WM + l31) * ROW, b_rd = NA * A_BYTES + (wn * WN + l31) * ROW;
+    const int l31 = lane & 31, lh = lane >> 5;
+    const int a_rd = (wm * WM + l31) * RA, a_sl = (lh ^ twist(l31, NA)) * 16, b_rd = A_BYTES + (wn * WN + l31) * RB, b_sl = (lh ^ twist(l31, NB)) * 16;
     struct Frags { half8 a[TM][NA], b[TN][NB]; };
     constexpr int READS = TM * NA + TN * NB, PRODS = (NA > 1) + (NB > 1) + 1, MMAS = PRODS * TM * TN;
     auto read = [&](int buf, int ks, int x, Frags& f) {      // fragment x of half ks of a chunk
-        const unsigned char* base = smem + buf * STAGE + ((2 * ks + lh) ^ swz) * 16;
-        if (x < TM * NA) f.a[x / NA][x % NA] = *reinterpret_cast<const half8*>(base + a_rd + (x % NA) * A_BYTES + (x / NA) * 32 * ROW);
-        else { const int y = x - TM * NA; f.b[y / NB][y % NB] = *reinterpret_cast<const half8*>(base + b_rd + (y % NB) * B_BYTES + (y / NB) * 32 * ROW); }
+        const unsigned char* base = smem + buf * STAGE;      // slot = half of the lane, half chunk, hi / lo: bits 0, 1, 2
+        if (x < TM * NA) f.a[x / NA][x % NA] = *reinterpret_cast<const half8*>(base + a_rd + (x / NA) * 32 * RA + (a_sl ^ (ks * 32 + (x % NA) * 64)));
+        else { const int y = x - TM * NA; f.b[y / NB][y % NB] = *reinterpret_cast<const half8*>(base + b_rd + (y / NB) * 32 * RB + (b_sl ^ (ks * 32 + (y % NB) * 64))); }
     };
     // The products of one half chunk, small terms first and neighbours on different accumulators, with the reads of the next half's fragments and
     // the loads of a later chunk spread between them: the matrix pipe is never without a product that is ready.
@@ -956,8 +956,8 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
                 for (int x = lane; x < E * E / 8; x += 64) {
                     const int c = x / (E / 8), r = (x % (E / 8)) * 8;
                     if (cb + c < d.m && rb + r < S.ld) {
-                        const unsigned char* q = S.hi + ((int64_t)(cb + c) * S.ld + rb + r) * 2;
-                        const uint4 h = *reinterpret_cast<const uint4*>(q), l = *reinterpret_cast<const uint4*>(q + S.step);
+                        const unsigned char* q = at_hi(S, cb + c, rb + r);
+                        const uint4 h = *reinterpret_cast<const uint4*>(q), l = *reinterpret_cast<const uint4*>(q + 64);
                         uint2* wh = reinterpret_cast<uint2*>(mine + c * LDH + r * 2);
                         uint2* wl = reinterpret_cast<uint2*>(lo + c * LDH + r * 2);
                         wh[0] = make_uint2(h.x, h.y); wh[1] = make_uint2(h.z, h.w);
@@ -999,7 +999,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
             for (int x = lane; x < E * E / 8; x += 64) {
                 const int c = x / (E / 8), r = (x % (E / 8)) * 8;
                 if (cb + c >= nc || rb + r >= T.ld) continue;
-                unsigned char* o = T.hi + ((int64_t)(cb + c) * T.ld + rb + r) * 2;
+                unsigned char* o = at_hi(T, cb + c, rb + r);
 #pragma unroll
                 for (int pl = 0; pl < 2; ++pl) {
                     const unsigned char* src = pl ? lo : mine;
@@ -1013,7 +1013,7 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
                                 w[k / 2] = (k & 1) ? (w[k / 2] & 0xffffu) | (v << 16) : (w[k / 2] & 0xffff0000u) | v;
                             }
                     }
-                    *reinterpret_cast<uint4*>(o + (pl ? T.step : 0)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(o + pl * 64) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
             if (half) continue;
@@ -1022,14 +1022,14 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
             for (int x = lane; x < E * E / 8; x += 64) {
                 const int r = x / (E / 8), c = (x % (E / 8)) * 8;
                 if (rb + r >= d.m || cb + c >= D.ld) continue;
-                unsigned char* o = D.hi + ((int64_t)(rb + r) * D.ld + cb + c) * 2;
+                unsigned char* o = at_hi(D, rb + r, cb + c);
 #pragma unroll
                 for (int pl = 0; pl < 2; ++pl) {
                     const unsigned char* src = pl ? lo : mine;
                     unsigned w[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) w[k] = at(src, c + 2 * k, r) | (unsigned)at(src, c + 2 * k + 1, r) << 16;
-                    *reinterpret_cast<uint4*>(o + (pl ? D.step : 0)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(o + pl * 64) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
         }
@@ -1112,8 +1112,8 @@ const char* check_mats(const wgs_matrix* mats, int count, int dtype, bool step, 
     if (steps < 1 || steps > MAX_STEPS) return "steps must be 1 .. 16";
     for (int i = 0; i < count; ++i) {
         const wgs_matrix& w = mats[i];
-        if (w.rows < 1 || w.cols < 1 || w.batch < 0 || (int64_t)w.rows * up(w.cols, BK) >= (1LL << 30) || (int64_t)w.cols * up(w.rows, BK) >= (1LL << 30))
-            return "bad sizes (rows, cols >= 1, fewer than 2^30 elements with the smaller side's padding to 32)";
+        if (w.rows < 1 || w.cols < 1 || w.batch < 0 || (int64_t)w.rows * up(w.cols, BK) >= (1LL << 29) || (int64_t)w.cols * up(w.rows, BK) >= (1LL << 29))
+            return "bad sizes (rows, cols >= 1, fewer than 2^29 elements with the smaller side's padding to 32)";
         if (w.in_row_stride < w.cols || w.out_row_stride < w.cols || w.in_row_stride >= (1LL << 31) || w.out_row_stride >= (1LL << 31)) return "row strides must be at least cols";
         if (w.batch > 1 && (w.in_batch_stride < 0 || w.out_batch_stride < (int64_t)(w.rows - 1) * w.out_row_stride + w.cols)) return "batch strides overlap";
         if (w.batch > (1 << 20)) return "batch must be at most 2^20";
