@@ -73,7 +73,10 @@ def phases_of(dtype, steps, step=False):
 def check(got, x, steps=5, coef=C3, eps=1e-7, dtype=None):
     dtype = dtype or x.dtype
     want = exact(x, steps, coef, eps)
-    model = (noisy(x, phases_of(dtype, steps), coef, eps) - want).square().sum((-2, -1)).sqrt()
+    # After many steps the error lies in few singular directions, and along one the size of a single draw of the noise is a |normal| variable: under
+    # a sixth of its scale once in 7.6 draws.  The root mean square of eight draws is not (P(chi2_8 / 8 < 1 / 36) < 1e-6).
+    draws = 8 if steps > 5 else 1
+    model = (sum((noisy(x, phases_of(dtype, steps), coef, eps, seed) - want).square().sum((-2, -1)) for seed in range(draws)) / draws).sqrt()
     size = want.square().sum((-2, -1)).sqrt()
     err = got.double() - want
     fro = err.square().sum((-2, -1)).sqrt()

@@ -703,14 +703,21 @@ __device__ __forceinline__ void tile_lower(int t, int tm, int& ti, int& tj) {
 template <int NA, int NB, int BM, int WAVES_M, int WAVES_N, int NS, int E, bool SPLIT = false>
 __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(const Jobs js, int total, int run, int most, int join, const Group g) {
     constexpr int BN = BM, NW = WAVES_M * WAVES_N, WM = BM / WAVES_M, WN = BN / WAVES_N, TM = WM / 32, TN = WN / 32;
-    constexpr int RA = NA * ROW, RB = NB * ROW, A_BYTES = BM * RA, B_BYTES = BN * RB, STAGE = A_BYTES + B_BYTES;      // bytes of a row, an operand, a chunk
-    constexpr int GA = 1024 / RA, GB = 1024 / RB, AI = BM / GA / NW, BI = BN / GB / NW, NPIECE = AI + BI;               // rows of a load, loads of a wave
+    constexpr int RA = NA * ROW, RB = NB * ROW, A_BYTES = BM * RA, B_BYTES = BN * RB, CHUNK = A_BYTES + B_BYTES;      // bytes of a row, an operand, a chunk
+    constexpr int KC = BM == 64 ? 2 : 1, STAGE = KC * CHUNK;                                                          // chunks of a stage
+    constexpr int GA = 1024 / RA, GB = 1024 / RB, AI = BM / GA / NW, BI = BN / GB / NW, CP = AI + BI, NPIECE = KC * CP;               // rows of a load, loads of a wave
     static_assert(AI * GA * NW == BM && BI * GB * NW == BN && TM * 32 * WAVES_M == BM && TN * 32 * WAVES_N == BN, "tile / wave count mismatch");
     static_assert(WM % E == 0 && WN % E == 0, "epilogue block");
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
 
+    // The arguments' lines all at once: read where they are needed, each would be a round trip to memory of its own.
+    {
+        const Mat& m0 = g.mat[0];
+        const Job& j0 = js.job[0];
+        asm volatile("" :: "s"(m0.M), "s"(m0.ws), "s"(m0.out), "s"(g.ws), "s"(g.info), "s"(js.sym), "s"(j0.kind), "s"(j0.first), "s"(js.job[1].kind), "s"(total));
+    }
     // Workgroups go round the 8 XCDs: runs of at most 32 tiles in turn, equally many each, so that an XCD's CUs work on neighbouring tiles and the
     // first entries (the longest sums) are spread over all XCDs.
     const int idx = (int)(blockIdx.x >> 3);
@@ -766,14 +773,16 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
     }
     // piece x of the next chunk (chunk nC, behind the last one that one again: its data is not used) into stage buf
     int nC = 0;
-    auto piece = [&](int buf, int x) {
-        const int c = k0 + (nC < nk ? nC : nk - 1);
-        lds_byte* st = (lds_byte*)(smem + buf * STAGE);
+    auto piece = [&](int buf, int y) {
+        const int x = y % CP, c1 = nC * KC + y / CP;
+        const bool past = KC == 2 && c1 >= nk;                  // (an odd number of chunks: zeros)
+        const int c = k0 + (c1 < nk ? c1 : nk - 1);
+        lds_byte* st = (lds_byte*)(smem + buf * STAGE + y / CP * CHUNK);
         if (x < AI) {
-            const int off = a_off[x];
+            const int off = past ? OOB : a_off[x];
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, st + (wave * AI + x) * 1024, 16, off, c * RA, 0, 0);
         } else {
-            const int off = b_off[x - AI];
+            const int off = past ? OOB : b_off[x - AI];
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, st + A_BYTES + (wave * BI + x - AI) * 1024, 16, off, c * RB, 0, 0);
         }
     };
@@ -834,11 +843,57 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
     const float isa = J.kind == POLY ? 1.f / info[I_SA + J.t] : 0.f;
     if (!SPLIT || !join) {
         landed(std::integral_constant<int, NS - 1>());
+        if (KC == 1)
 #pragma unroll
-        for (int x = 0; x < READS; ++x) read(0, 0, x, f0);
+            for (int x = 0; x < READS; ++x) read(0, 0, x, f0);
     }
     int cur = 0;
-    for (int kt = 0; kt < (SPLIT && join ? 0 : nk); ++kt) {
+    if constexpr (KC == 2) {
+        // One 32 x 32 block a wave: three products a half chunk, over before a fragment read or a barrier is.  So a stage of two chunks at a time: its
+        // four halves' fragments are read under the products of the stage before, cross terms into an accumulator of their own.
+        static_assert(TM == 1 && TN == 1, "one block a wave");
+        Frags e[4], o[4];
+        f32x16 cross;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) cross[r] = 0.f;
+        auto read4 = [&](int buf, int x, Frags (&f)[4]) {
+            const unsigned char* base = smem + buf * STAGE + (x >> 1) * CHUNK;
+#pragma unroll
+            for (int pl = 0; pl < NA; ++pl) f[x].a[0][pl] = *reinterpret_cast<const half8*>(base + a_rd + (a_sl ^ ((x & 1) * 32 + pl * 64)));
+#pragma unroll
+            for (int pl = 0; pl < NB; ++pl) f[x].b[0][pl] = *reinterpret_cast<const half8*>(base + b_rd + (b_sl ^ ((x & 1) * 32 + pl * 64)));
+        };
+        auto mma4 = [&](const Frags& f) {
+            if (NA > 1) cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[0][NA - 1], f.b[0][0], cross, 0, 0, 0);
+            acc[0][0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[0][0], f.b[0][0], acc[0][0], 0, 0, 0);
+            if (NB > 1) cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.a[0][0], f.b[0][NB - 1], cross, 0, 0, 0);
+        };
+        auto step = [&](const Frags (&f)[4], Frags (&nf)[4]) {
+            landed(std::integral_constant<int, NS - 2>());          // the next stage; this one's fragments are in registers
+            const int old = cur;
+            cur = cur + 1 == NS ? 0 : cur + 1;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                read4(cur, h, nf);
+#pragma unroll
+                for (int x = h * NPIECE / 4; x < (h + 1) * NPIECE / 4; ++x) piece(old, x);
+                mma4(f[h]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            ++nC;
+        };
+        const int stages = SPLIT && join ? 0 : (nk + 1) / 2;
+        if (!SPLIT || !join)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) read4(0, h, e);
+        for (int t = 0; t < stages; t += 2) {                   // (a stage behind the last one is zeros)
+            step(e, o);
+            step(o, e);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[0][0][r] += cross[r];
+    } else
+    for (int kt = 0; kt < nk; ++kt) {
         ORTHO_MMA(f0, f1, cur, 1, 0, 0)
         landed(std::integral_constant<int, NS - 2>());
         const int old = cur;
@@ -1160,7 +1215,7 @@ int ceil_log2(double v) { int e; const double f = frexp(v, &e); return f == 0.5 
 
 template <int NA, int NB, int BM, int WM, int WN, int NS, int E, bool SPLIT = false>
 void launch_gemm(const Group& g, const Jobs& js, int total, hipStream_t st, int most = 1, int join = 0) {
-    constexpr int stages = NS * (NA + NB) * BM * ROW, blocks = WM * WN * E * (E + 4) * 4;
+    constexpr int stages = NS * (BM == 64 ? 2 : 1) * (NA + NB) * BM * ROW, blocks = WM * WN * E * (E + 4) * 4;
     constexpr int sm = stages > blocks ? stages : blocks;
     static_assert(sm <= 160 * 1024, "LDS of a CU");
     auto k = ortho_gemm_kernel<NA, NB, BM, WM, WN, NS, E, SPLIT>;
@@ -1208,11 +1263,11 @@ int gemm(const Group& g, const Jobs& js, hipStream_t st) {
         if (g.part && js.count == 1 && total <= 128)
             for (int x = 2; x <= 16 && tiles_of(g, js, 64, x) <= 768; ++x) most = x;
         if (longest - longest / parts_of_sum(longest, most) > 40) {
-            launch_gemm<NA, NB, 64, 2, 2, 4, 32, true>(g, js, tiles_of(g, js, 64, most), st, most);
-            launch_gemm<NA, NB, 64, 2, 2, 4, 32, true>(g, js, total, st, most, 1);
-        } else launch_gemm<NA, NB, 64, 2, 2, 8, 32>(g, js, total, st);
+            launch_gemm<NA, NB, 64, 2, 2, 2, 32, true>(g, js, tiles_of(g, js, 64, most), st, most);
+            launch_gemm<NA, NB, 64, 2, 2, 2, 32, true>(g, js, total, st, most, 1);
+        } else launch_gemm<NA, NB, 64, 2, 2, 4, 32>(g, js, total, st);
     }
-    else launch_gemm<NA, NB, 64, 2, 2, 4, 32>(g, js, total, st);
+    else launch_gemm<NA, NB, 64, 2, 2, 2, 32>(g, js, total, st);
     return WGS_OK;
 }
 
