@@ -329,9 +329,23 @@ def test_refusals(dev):
         ops.orthogonalise([x, x.half()])
     m = torch.zeros(4, 5, device=dev)
     with pytest.raises(L.WgsError, match='twice'):
-        ops.muon_step([x, x], [x, x], [m, m.clone()], 0.1)
+        ops.muon_step([x, x], [x.clone(), x.clone()], [m, m.clone()], 0.1)
+    with pytest.raises(L.WgsError, match='overlaps'):
+        ops.muon_step([x], [x], [m], 0.1)                                   # a gradient that is the weight
+    with pytest.raises(L.WgsError, match='overlaps'):
+        ops.muon_step([x], [m], [m], 0.1)
+    big = torch.randn(12, 5, device=dev)
+    with pytest.raises(L.WgsError, match='overlaps'):
+        ops.muon_step([big[:8], big[6:10]], [torch.randn(8, 5, device=dev), x], [torch.zeros(8, 5, device=dev), m], 0.1)
+    w = torch.nn.Parameter(x.clone())
+    plan = ops.MuonUpdate([w], [x], [m])
+    plan.step(0.1)
+    w.data = w.data.clone()
+    with pytest.raises(L.WgsError, match='other memory'):
+        plan.step(0.1)
+    g = x.clone()
     with pytest.raises(L.WgsError, match='momentum must be'):
-        ops.muon_step([x], [x], [m], 0.1, momentum=1.0)
+        ops.muon_step([x], [g], [m], 0.1, momentum=1.0)
     with pytest.raises(L.WgsError, match='a momentum must be'):
         ops.muon_step([x], [x], [m.half()], 0.1)
     with pytest.raises(L.WgsError, match='elements of a row'):

@@ -139,6 +139,27 @@ def _rows_of(x):
     return x, (x.stride(0) if x.shape[0] > 1 else V)
 
 
+_P, _I, _I64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
+_logprob_calls = None
+
+
+def _logprobs():
+    """(workspace, forward, backward) entry points with their argument types: plain integers go in without a conversion object each."""
+    global _logprob_calls
+    if _logprob_calls is None:
+        lib = L.lib()
+        ws, fwd, bwd = lib.wgs_label_logprobs_ws_bytes, lib.wgs_label_logprobs_fwd, lib.wgs_label_logprobs_bwd
+        ws.argtypes = [_I64, _I64, _I]
+        fwd.argtypes = [_P, _I, _I64, _I64, _I64, _P, _I64, _I, _P, _P, _P, _P, _P, _P, _I64, _P]
+        bwd.argtypes = [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _P]
+        _logprob_calls = ws, fwd, bwd
+    return _logprob_calls
+
+
+def _upstream(g):
+    return g if g is None or (g.dtype == torch.float32 and g.is_contiguous()) else g.to(torch.float32).contiguous()
+
+
 class _LabelLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, top, ignore_index):
@@ -147,18 +168,17 @@ class _LabelLogprobsFn(torch.autograd.Function):
         rows = x.shape[0]
         code = _DTYPES[x.dtype]
         lead = logits.shape[:-1]
+        ws_bytes, fwd, _ = _logprobs()
         with _on(dev):
             logp = torch.empty(lead, device=dev)
             entropy = torch.empty(lead, device=dev)
             stat = torch.empty(rows, 2, device=dev)
             top_logp = torch.empty(lead + (top,), device=dev)
             top_index = torch.empty(lead + (top,), dtype=torch.int64, device=dev)
-            need = L.lib().wgs_label_logprobs_ws_bytes(L.c_int64(rows), L.c_int64(V), top)
+            need = ws_bytes(rows, V, top)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            L.check(L.lib().wgs_label_logprobs_fwd(L.rawptr(x), code, L.c_int64(rows), L.c_int64(V), L.c_int64(stride), L.rawptr(labels),
-                                                   L.c_int64(ignore_index), top, L.rawptr(logp), L.rawptr(entropy), L.rawptr(stat),
-                                                   L.rawptr(top_logp), L.rawptr(top_index), L.rawptr(ws), L.c_int64(need), L.stream()),
-                    'wgs_label_logprobs_fwd')
+            L.check(fwd(x.data_ptr(), code, rows, V, stride, labels.data_ptr(), ignore_index, top, logp.data_ptr(), entropy.data_ptr(), stat.data_ptr(),
+                        top_logp.data_ptr(), top_index.data_ptr(), ws.data_ptr() if need else None, need, L.stream_id()), 'wgs_label_logprobs_fwd')
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_index)
         # (a copy made of a strided input is saved in its place)
@@ -175,18 +195,19 @@ class _LabelLogprobsFn(torch.autograd.Function):
         x, stride = _rows_of(logits)
         rows, size = x.shape[0], x.element_size()
         with _on(dev):
-            up = [None if g is None else g.to(torch.float32).contiguous() for g in (g_logp, g_entropy, g_top)]
+            g_logp, g_entropy, g_top = _upstream(g_logp), _upstream(g_entropy), _upstream(g_top)
             # rows of the gradient start at the same place of a 16-byte block as those of the logits: whole-vector reads and writes
-            per = 16 // size
             first = x.data_ptr() % 16 // size
-            gstride = V + (stride - V) % per if rows > 1 else V
-            buf = torch.empty(first + rows * gstride, dtype=x.dtype, device=dev)
-            grad = buf[first:].view(rows, gstride)[:, :V]
-            L.check(L.lib().wgs_label_logprobs_bwd(L.rawptr(x), _DTYPES[x.dtype], L.c_int64(rows), L.c_int64(V), L.c_int64(stride),
-                                                   L.rawptr(labels), L.c_int64(ignore_index), L.rawptr(stat), L.rawptr(entropy), top,
-                                                   L.rawptr(top_index), L.rawptr(up[0]), L.rawptr(up[1]), L.rawptr(up[2]),
-                                                   L.rawptr(grad), L.c_int64(gstride), L.stream()), 'wgs_label_logprobs_bwd')
-        return grad.view(shape) if len(shape) != 2 and gstride == V else grad.reshape(shape), None, None, None
+            gstride = V + (stride - V) % (16 // size) if rows > 1 else V
+            if first == 0 and gstride == V:
+                grad = torch.empty(shape, dtype=x.dtype, device=dev)
+            else:
+                grad = torch.empty(first + rows * gstride, dtype=x.dtype, device=dev)[first:].view(rows, gstride)[:, :V]
+            L.check(_logprobs()[2](x.data_ptr(), _DTYPES[x.dtype], rows, V, stride, labels.data_ptr(), ignore_index, stat.data_ptr(), entropy.data_ptr(),
+                                   top, top_index.data_ptr(), None if g_logp is None else g_logp.data_ptr(),
+                                   None if g_entropy is None else g_entropy.data_ptr(), None if g_top is None else g_top.data_ptr(),
+                                   grad.data_ptr(), gstride, L.stream_id()), 'wgs_label_logprobs_bwd')
+        return (grad if grad.shape == shape else grad.reshape(shape)), None, None, None
 
 
 def label_logprobs(logits, labels, top=0, ignore_index=-100):
@@ -354,19 +375,26 @@ class MuonUpdate:
                 if (N > 1 and t.stride(1) != 1) or (M > 1 and t.stride(0) < N):
                     raise L.WgsError("%s: the elements of a row must be adjacent, got strides %s" % (what, t.stride()))
             gr, wr = (g2.stride(0), w2.stride(0)) if M > 1 else (N, N)
-            spans.append((m2.data_ptr(), m2.data_ptr() + 4 * M * N, True))
-            spans.append((w2.data_ptr(), w2.data_ptr() + w2.element_size() * ((M - 1) * wr + N), wr == N))
+            spans.append((m2.data_ptr(), m2.data_ptr() + 4 * M * N, True, True))
+            spans.append((w2.data_ptr(), w2.data_ptr() + w2.element_size() * ((M - 1) * wr + N), wr == N, True))
+            spans.append((g2.data_ptr(), g2.data_ptr() + g2.element_size() * ((M - 1) * gr + N), gr == N, False))
             self.factors.append(max(1.0, M / N) ** 0.5 if scale is None else 0.2 * max(M, N) ** 0.5 if scale == 'rms' else float(scale))
             _MATRIX.pack_into(self.mats, k * _MATRIX.size, g2.data_ptr(), w2.data_ptr(), m2.data_ptr(), 0, 0, gr, wr, M, N, 1, 0.0, 1.0, 0)
         _check_apart(spans)
         self.code = _DTYPES[dtype]
         self.need = L.lib().wgs_muon_step_ws_bytes(self.mats, self.n, self.code, self.steps)
+        self.places = self._places()
         self.lr = None
+
+    def _places(self):
+        return [t.data_ptr() for ts in self.tensors for t in ts]
 
     @torch.no_grad()
     def step(self, lr):
         if not self.n:
             return
+        if self._places() != self.places:
+            raise L.WgsError("MuonUpdate: a tensor has been given other memory since it was described: make a new one")
         if lr != self.lr:
             decay = 1.0 - lr * self.weight_decay
             for k, f in enumerate(self.factors):
@@ -382,12 +410,16 @@ _STEP_DECAY, _STEP_DECAY_AT = struct.Struct('=2f'), struct.calcsize('=3Q4q3i')
 
 
 def _check_apart(spans):
-    """What a step writes may not overlap: spans (start, end, dense) in bytes.  A span that begins inside a dense one overlaps it; inside a strided
-    one it may lie between the rows."""
-    spans = sorted(spans)
-    for (a0, a1, dense), (b0, _, _) in zip(spans, spans[1:]):
-        if b0 == a0 or (dense and b0 < a1):
-            raise L.WgsError("muon_step: a param or momentum is given twice, or overlaps another")
+    """What a step writes may overlap neither what else it writes nor the gradients: spans (start, end, dense, written) in bytes.  A span that
+    begins inside a dense one overlaps it; inside a strided one it may lie between the rows."""
+    end = {True: 0, False: 0}                   # of the dense spans so far, written and read
+    start = {True: -1, False: -1}
+    for a, b, dense, written in sorted(spans):
+        if a < end[True] or a == start[True] or (written and (a < end[False] or a == start[False])):
+            raise L.WgsError("muon_step: a param or momentum is given twice, or overlaps another tensor of the call")
+        start[written] = a
+        if dense:
+            end[written] = max(end[written], b)
 
 
 def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, grad_scale=1.0, steps=5,
