@@ -609,10 +609,12 @@ int wgs_label_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t 
  *     out <- decay out - step * (X_steps of u)       (in = gradient, out = weight; decay = 1 - lr weight_decay, step = lr * the shape's factor)
  * Any number of matrices of any sizes goes through the same few launches.  in / out of dtype, rows `row_stride` apart (elements within a row
  * adjacent), `batch` instances `batch_stride` apart (in: 0 repeats one); momentum fp32 [batch, rows, cols] contiguous (wgs_muon_step only).
- * The matrices of a call may not overlap where they are written; in == out is allowed.  rows * cols (padded to 32) < 2^30.
+ * What is written may not overlap anything else of the call; in == out is allowed (wgs_orthogonalise).  rows * cols (the smaller side padded
+ * to 32) < 2^29.
  * steps 1 .. 16; coefficients whose iterates leave 1e6 are refused.  Differentiable it is not.
- * ws: *_ws_bytes() of the same matrices (pointers may be NULL in that call's batch = 0 entries only), 256-byte aligned; contents do not matter
- * before or after the call.
+ * Singular values are reached in fp32's precision (fp16 hi + lo operands, fp32 sums, fp64 norms); how many iterations are joined on the smaller
+ * side's matrices goes by the result's type.
+ * ws: *_ws_bytes() of the same matrices, 256-byte aligned; contents do not matter before or after the call.
  */
 typedef struct wgs_matrix {
     const void* in;
