@@ -690,7 +690,7 @@ def main():
             _T4.TrainStep.tail_pause_res_default, _T4.TrainStep.tail_hook_res_default = int(_pr), int(_hr)
     if os.environ.get('WGS_RGB') == '0':             # development A/B: ToRGB as its own launch everywhere
         C.RGB_FUSED = False
-    if os.environ.get('WGS_PRIO') == '0':            # development A/B: no high-priority stream for the step's critical path
+    if os.environ.get('WGS_PRIO') == '0':            # development A/B: no stream of its own for the step's critical path
         ENGINE_KW['priority_main'] = False
     if os.environ.get('WGS_FWD_PLANE') == '0':       # development A/B: forward fp16 planes off (conv.FWD_PLANE)
         C.FWD_PLANE = False

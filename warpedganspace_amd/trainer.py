@@ -68,13 +68,13 @@ _STREAMS = {}
 
 
 def _engine_streams(device):
-    """(side, prefetch, high-priority main) streams of `device`, created once per process."""
+    """(side, prefetch, main) streams of `device`, created once per process."""
     key = torch.device(device).index if torch.device(device).index is not None else torch.cuda.current_device()
     if key not in _STREAMS:
         # (CU-masked side streams — hipExtStreamCreateWithCUMask, 3/4 or 1/2 of every XCD's CUs, so that the critical path's short
         # launches always find free CUs — measured slower both for all side work (auto 25.7 -> 26.7 / 30.0 ms, fp32w 53.7 -> 59.9 / 69.9)
         # and for the prefetched pass's middle stage alone, the one that runs beside the Reconstructor (auto 25.7 -> 26.5 / 38.9 ms))
-        _STREAMS[key] = (torch.cuda.Stream(device=device), torch.cuda.Stream(device=device), torch.cuda.Stream(device=device, priority=-1))
+        _STREAMS[key] = (torch.cuda.Stream(device=device), torch.cuda.Stream(device=device), torch.cuda.Stream(device=device))
     return _STREAMS[key]
 
 
@@ -165,11 +165,10 @@ class TrainStep:
         # three streams put the fourth engine's "concurrent" streams on ONE queue — bench.py's second engine ran 37.5 instead of
         # 27.5 ms per step.  The streams are per device, shared by all engines.
         self.side_stream, self.pre_stream, main_stream = _engine_streams(device)
-        # The step's critical path (shifted forward -> R -> loss -> R backward -> G backward -> Adam) runs on a HIGH-priority stream of
-        # its own; the side work that only has to be finished by the end of the step (the un-shifted pass of this / the next batch,
-        # R's weight gradients) stays on default-priority streams: when a CU frees up, the critical path's next workgroups — the
-        # Reconstructor's ~300 short launches in particular — are dispatched ahead of the side streams' long-running generator tiles
-        # instead of queueing behind them.
+        # The step's critical path (shifted forward -> R -> loss -> R backward -> G backward -> Adam) runs on a stream of its own, the side work
+        # that only has to be finished by the end of the step (the un-shifted pass of this / the next batch, R's weight gradients) on others.
+        # All have the default priority: work on streams of different priorities can wait for good, and a higher one for this stream was worth
+        # 0.3 % of the rate (1318.8 against 1315.0 img/s).
         self.main_stream = main_stream if (priority_main and two_streams) else None
         self.two_streams = two_streams       # un-shifted generator pass on the side stream
         self.defer_wgrad = defer_wgrad       # R's weight gradients on the side stream, next to the generator's backward
@@ -412,7 +411,7 @@ class TrainStep:
         return z, idx, mag
 
     def step(self, z=None, idx=None, mag=None):
-        """One training step.  Enqueues on the engine's high-priority stream (ordered after the caller's current stream, which in turn
+        """One training step.  Enqueues on the engine's own stream (ordered after the caller's current stream, which in turn
         waits for the step: the caller sees ordinary stream semantics) or, without it, on the current stream."""
         if self.main_stream is None or not self.two_streams:
             return self._step(z, idx, mag)
