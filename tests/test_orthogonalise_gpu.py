@@ -132,6 +132,22 @@ def test_spectra(dev, dtype, kind, shape):
     check(ops.orthogonalise(x), x)
 
 
+@DT
+@pytest.mark.parametrize('steps', [2, 3, 5, 8])
+@pytest.mark.parametrize('shape', [(33, 4100), (2, 64, 2500), (66, 66), (3, 97, 101), (128, 128), (2, 300, 120)], ids=str)
+def test_few_rows(dev, dtype, steps, shape):
+    x = matrices(dev, shape, dtype, 3, 'rows')
+    check(ops.orthogonalise(x, steps=steps), x, steps)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=['bf16', 'f16'])
+@pytest.mark.parametrize('shapes', [[(33, 4100), (2, 128, 140), (1, 2500), (90, 3)], [(1, 4100), (31, 2100), (2, 64, 2049)], [(128, 300), (129, 300)]], ids=str)
+def test_few_rows_together(dev, dtype, shapes):
+    xs = [matrices(dev, s, dtype, i) for i, s in enumerate(shapes)]
+    for got, x in zip(ops.orthogonalise(xs), xs):
+        check(got, x)
+
+
 @pytest.mark.parametrize('steps', [1, 2, 3, 4, 6, 7, 11, 16])
 @DT
 def test_steps_and_coefficients(dev, dtype, steps):

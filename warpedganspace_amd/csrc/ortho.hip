@@ -1090,11 +1090,200 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
         }
 }
 
+// ---- 4. a whole phase's polynomial for m <= 128, one workgroup a matrix -----------------------------------------------------------------------------
+// From the Gram matrix A (read once) to Q (written once): per iteration B = aI + bA + cA^2, P = B A beside Q <- B Q, A = P B, with A (or P) and B in
+// LDS as hi and lo planes and Q in registers: a wave a block of 32 columns, whose result layout is the next product's operand (as in the small
+// kernel).  Symmetric products: the tiles on and under the diagonal, written twice.  Some 14 us an iteration at
+// m = 128 (the latency of its dependent products and LDS) instead of three launches of some 9: 64 x 128x512 fp16 176 -> 132 us, one in bf16 158 -> 91.
+constexpr int CHAIN_M = 128;
+struct ChainArgs { int t0, len, src, dst; float a, b, c; float sb[MAX_STEPS], grow[MAX_STEPS], sq[MAX_STEPS]; };      // grow: 2^ceil log2 of B's bound; sq: Q' scale / (Q scale sb)
+template <int MT>
+__global__ __launch_bounds__(512, 1) void ortho_chain_kernel(const Group g, const ChainArgs ar) {
+    constexpr int S = 32 * MT, LD = S + 8, TRI = MT * (MT + 1) / 2;
+    typedef _Float16 plane_t[S][LD];
+    __shared__ __attribute__((aligned(16))) plane_t la[2], lb[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, lh = lane >> 5;
+    const Mat& mat = g.mat[entry_of(g, blockIdx.x)];
+    const int b = blockIdx.x - mat.first;
+    const Dims d = dims_of(mat.M, mat.N);
+    const float* info = info_of(g, blockIdx.x);
+    const Plane A = plane_of(g, mat, d, b, ar.src), Q = plane_of(g, mat, d, b, ar.dst);
+
+    for (int e = tid; e < S * (S / 8); e += 512) {
+        const int r = e / (S / 8), c = (e % (S / 8)) * 8;
+        uint4 h = make_uint4(0, 0, 0, 0), l = h;
+        if (r < d.m && c < d.mp) { h = *reinterpret_cast<const uint4*>(at_hi(A, r, c)); l = *reinterpret_cast<const uint4*>(at_hi(A, r, c) + 64); }
+        *reinterpret_cast<uint4*>(&la[0][r][c]) = h;
+        *reinterpret_cast<uint4*>(&la[1][r][c]) = l;
+    }
+    auto place = [](int t, int& p, int& q) { p = 0; while (t > p) { t -= p + 1; ++p; } q = t; };
+    auto product = [&](const plane_t (&x)[2], const plane_t (&y)[2], int p, int q) {      // rows of tile p of x times rows of tile q of y
+        f32x16 s, w;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) { s[k] = 0.f; w[k] = 0.f; }
+#pragma unroll
+        for (int ks = 0; ks < 2 * MT; ++ks) {
+            const int kc = 16 * ks + 8 * lh;
+            const half8 ah = *reinterpret_cast<const half8*>(&x[0][32 * p + l31][kc]), al = *reinterpret_cast<const half8*>(&x[1][32 * p + l31][kc]);
+            const half8 bh = *reinterpret_cast<const half8*>(&y[0][32 * q + l31][kc]), bl = *reinterpret_cast<const half8*>(&y[1][32 * q + l31][kc]);
+            w = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, w, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, s, 0, 0, 0);
+            w = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, w, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) s[k] += w[k];
+        return s;
+    };
+    auto put = [&](plane_t (&x)[2], int p, int q, int k4, float (&v)[4]) {      // elements 4 k4 .. + 3 of tile (p, q), rows r .. r + 3 of a column, and their mirror
+        const int r = 32 * p + 8 * k4 + 4 * lh, c = 32 * q + l31;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (r + k >= d.m || c >= d.m) v[k] = 0.f;
+        half4 h, l;
+        split_many<4>(v, h, l);
+        _Float16 *dh = &x[0][r][c], *dl = &x[1][r][c], *mh = &x[0][c][r], *ml = &x[1][c][r];
+        if (p != q) {
+            *reinterpret_cast<half4*>(mh) = h;
+            *reinterpret_cast<half4*>(ml) = l;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { dh[k * LD] = h[k]; dl[k * LD] = l[k]; }
+        } else {                                                                   // not the strict upper triangle of a diagonal tile
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (r + k >= c) { dh[k * LD] = h[k]; dl[k * LD] = l[k]; mh[k] = h[k]; ml[k] = l[k]; }
+        }
+    };
+    frag qh[MT][2], ql[MT][2];          // waves 0 .. 3: Q's columns 32 wave ..: lane = column, 8 rows a fragment
+    __syncthreads();
+    for (int it = 0; it < ar.len; ++it) {
+        const int t = ar.t0 + it;
+        const float sA = info[I_SA + t], isa = 1.f / sA, sb = ar.sb[it];
+        const bool last = it + 1 == ar.len;
+        for (int e = wave; e < TRI; e += 8) {
+            int p, q;
+            place(e, p, q);
+            const f32x16 s = product(la, la, p, q);
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4) {
+                const int r = 32 * p + 8 * k4 + 4 * lh, c = 32 * q + l31;
+                const half4 h = *reinterpret_cast<const half4*>(&la[0][c][r]), l = *reinterpret_cast<const half4*>(&la[1][c][r]);      // A by symmetry
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    v[k] = ((r + k == c ? ar.a : 0.f) + (ar.b * (((float)h[k] + (float)l[k]) * isa) + ar.c * (s[4 * k4 + k] * isa * isa))) * sb;
+                put(lb, p, q, k4, v);
+            }
+        }
+        __syncthreads();
+        f32x16 acc[3];
+        if (wave >= 4) {
+            if (!last)
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (wave - 4 + 4 * i < TRI) {
+                        int p, q;
+                        place(wave - 4 + 4 * i, p, q);
+                        acc[i] = product(lb, la, p, q);
+                    }
+        } else if (wave < MT) {
+            auto pick = [&](int pl, int row, int k0) {          // 8 values of a row of B in the order of a result's rows
+                const int2 u = *reinterpret_cast<const int2*>(&lb[pl][row][k0 + 4 * lh]), w = *reinterpret_cast<const int2*>(&lb[pl][row][k0 + 4 * lh + 8]);
+                return frag{u.x, u.y, w.x, w.y};
+            };
+            if (it == 0) {
+#pragma unroll
+                for (int u = 0; u < MT; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) { qh[u][h] = pick(0, 32 * wave + l31, 32 * u + 16 * h); ql[u][h] = pick(1, 32 * wave + l31, 32 * u + 16 * h); }
+            } else {
+                f32x16 s[MT];
+#pragma unroll
+                for (int u = 0; u < MT; ++u) {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) s[u][k] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < 2 * MT; ++ks) {
+                        const half8 bh = __builtin_bit_cast(half8, pick(0, 32 * u + l31, 16 * ks)), bl = __builtin_bit_cast(half8, pick(1, 32 * u + l31, 16 * ks));
+                        const half8 vh = __builtin_bit_cast(half8, qh[ks >> 1][ks & 1]), vl = __builtin_bit_cast(half8, ql[ks >> 1][ks & 1]);
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl, vh, s[u], 0, 0, 0);
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, vl, s[u], 0, 0, 0);
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh, vh, s[u], 0, 0, 0);
+                    }
+                }
+                const float f = ar.sq[it];
+#pragma unroll
+                for (int u = 0; u < MT; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[8];
+                        half8 x, y;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = s[u][8 * h + k] * f;
+                        split_many<8>(v, x, y);
+                        qh[u][h] = __builtin_bit_cast(frag, x); ql[u][h] = __builtin_bit_cast(frag, y);
+                    }
+            }
+        }
+        if (last) break;
+        __syncthreads();
+        if (wave >= 4) {
+            const float f = 1.f / (ar.grow[it] * sb);
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (wave - 4 + 4 * i < TRI) {
+                    int p, q;
+                    place(wave - 4 + 4 * i, p, q);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float v[4] = {acc[i][4 * k] * f, acc[i][4 * k + 1] * f, acc[i][4 * k + 2] * f, acc[i][4 * k + 3] * f};
+                        put(la, p, q, k, v);
+                    }
+                }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (wave + 8 * i < TRI) {
+                int p, q;
+                place(wave + 8 * i, p, q);
+                acc[i] = product(la, lb, p, q);
+            }
+        __syncthreads();
+        const float f = ar.grow[it] / sb * (info[I_SA + t + 1] / sA);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (wave + 8 * i < TRI) {
+                int p, q;
+                place(wave + 8 * i, p, q);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float v[4] = {acc[i][4 * k] * f, acc[i][4 * k + 1] * f, acc[i][4 * k + 2] * f, acc[i][4 * k + 3] * f};
+                    put(la, p, q, k, v);
+                }
+            }
+        __syncthreads();
+    }
+    const int row = 32 * wave + l31;          // Q is symmetric: a lane's column is a row
+    if (wave < MT && row < d.m)
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int k = 32 * u + 16 * h + 8 * x + 4 * lh;
+                    if (k < d.mp) {
+                        *reinterpret_cast<int2*>(at_hi(Q, row, k)) = make_int2(qh[u][h][2 * x], qh[u][h][2 * x + 1]);
+                        *reinterpret_cast<int2*>(at_hi(Q, row, k) + 64) = make_int2(ql[u][h][2 * x], ql[u][h][2 * x + 1]);
+                    }
+                }
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------
 struct Plan { int phases, len[MAX_STEPS]; int planes, npx, nt, ns; };
 // Iterations of a phase.  Longer phases leave out products with the n columns, but A_t then carries its own rounding through a^2 a step instead
-// of being formed anew from X_t: measured on spectra from flat to a single spike, one phase of five is within 4e-4 of the exact factor, (3, 2)
-// within 3e-5, single iterations within the 32-bit iteration's own 2e-5 (1e-6 .. 1e-5 for noise-dominated matrices).  So: what the result's
+// of being formed anew from X_t: measured on spectra from flat to a single spike, one phase of five is within 5e-4 of the exact factor, (3, 2)
+// within 5e-5, single iterations within the 32-bit iteration's own 3e-5 (1e-6 .. 1e-5 for noise-dominated matrices).  So: what the result's
 // type can hold.
 Plan plan_of(int dtype, bool step, int steps) {
     Plan p;
@@ -1336,6 +1525,8 @@ int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step
             else if (dtype == WGS_BF16) launch_prepare<WGS_BF16, false>(g, mo, bd, st);
             else launch_prepare<WGS_F16, false>(g, mo, bd, st);
         }
+        int chained = 0;                     // the largest m
+        for (int i = 0; i < g.count; ++i) { const int m = dims_of(g.mat[i].M, g.mat[i].N).m; if (m > chained) chained = m; }
         int t = 0;
         for (int ph = 0; ph < p.phases; ++ph) {
             const bool single = ph == 0 && p.planes == 1;
@@ -1355,6 +1546,21 @@ int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step
             if (rc) return rc;
             js.kgram = 0;
             double sq = 1.0;
+            if (p.len[ph] > 1 && chained <= CHAIN_M) {
+                ChainArgs ca = {};
+                ca.t0 = t; ca.len = p.len[ph]; ca.src = A; ca.dst = Q; ca.a = (float)a; ca.b = (float)b; ca.c = (float)c;
+                double bound = 1.0;
+                for (int it = 0; it < p.len[ph]; ++it, ++t) {
+                    const int em = ceil_log2(q[t]);
+                    const double sb = ldexp(1.0, 14 - em);
+                    bound *= q[t];
+                    const double sq2 = it ? ldexp(1.0, 14 - ceil_log2(bound)) : sb;
+                    ca.sb[it] = (float)sb; ca.grow[it] = (float)ldexp(1.0, em); ca.sq[it] = (float)(sq2 / (sq * sb));
+                    sq = sq2;
+                }
+                if (chained <= 64) WGS_LAUNCH(ortho_chain_kernel<2>, dim3((unsigned)g.instances), dim3(512), 0, st, g, ca);
+                else WGS_LAUNCH(ortho_chain_kernel<4>, dim3((unsigned)g.instances), dim3(512), 0, st, g, ca);
+            } else
             for (int it = 0; it < p.len[ph]; ++it, ++t) {
                 const int em = ceil_log2(q[t]);
                 const double sb = ldexp(1.0, 14 - em);
