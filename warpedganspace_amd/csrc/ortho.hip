@@ -1468,11 +1468,17 @@ void launch_prepare(const Group& g, const Momentum& mo, const Bounds& bd, hipStr
     WGS_LAUNCH((ortho_split_kernel<DT, STEP>), dim3((unsigned)tiles), dim3(256), 0, st, g, mo, bd, (int)tiles);
 }
 
-bool all_small(const Group& g) {
-    // one workgroup a matrix: beyond some 1024 columns a few matrices are done sooner by the general path's many (64 x 2000 fp32: 245 against some 160 us)
+bool all_small(const Group& g, const Plan& p, int steps) {
+    // One workgroup a matrix takes some (5 + 0.022 n) us a step at m = 64, the general path's many workgroups are done sooner with long rows.  Single
+    // iterations: where there are few matrices of over 1024 columns (64 x 2000 fp32: 245 against some 160 us).  Joined ones, with the chain kernel: m > 32
+    // from some 640 phases / steps columns (one of 64 x 64 bf16 40 against 45 us, 64 x 256 61 / 47, 64 x 1000 142 / 51, 512 of them 396 / 196; fp16, two
+    // phases: 64 x 64 40 / 60, 64 x 256 61 / 64, 64 x 576 98 / 67), m <= 32 like single ones (32 x 256 bf16 27 / 47, 32 x 2000 95 / 55).
+    const bool joined = p.phases < steps;
     for (int i = 0; i < g.count; ++i) {
         const Dims d = dims_of(g.mat[i].M, g.mat[i].N);
-        if (!is_small(d) || (d.m > 32 && d.n > 1024 && g.instances < 32)) return false;
+        if (!is_small(d)) return false;
+        if (joined && d.m > 32 && d.n * steps > 640 * p.phases) return false;
+        if ((joined || d.m > 32) && d.n > 1024 && g.instances < 32) return false;
     }
     return true;
 }
@@ -1512,7 +1518,7 @@ int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step
     sm.bd = bd; sm.a = (float)a; sm.b = (float)b; sm.c = (float)c;
     for (int t = 0; t < steps; ++t) sm.sb[t] = (float)ldexp(1.0, 14 - ceil_log2(q[t]));
     while (next_chunk(mats, count, p, cur, g) > 0) {
-        if (all_small(g)) {
+        if (all_small(g, p, steps)) {
             launch_small(g, mo, sm, st);
             continue;
         }
