@@ -283,6 +283,28 @@ def test_muon_step_on_convolution_weights(dev):
     assert b[0].is_contiguous(memory_format=torch.channels_last)
 
 
+def test_muon_step_on_pointwise_weights(dev):
+    """A 1 x 1 convolution's gradient may carry other strides in its single-entry dimensions."""
+    w, g, m = (matrices(dev, (24, 40, 1, 1), torch.float32, k) for k in range(3))
+    a = [t.clone() for t in (w, g, m)]
+    b = [w.clone(), g.clone().as_strided(g.shape, (40, 1, 40, 40)), m.clone()]
+    ops.muon_step([a[0]], [a[1]], [a[2]], 0.1)
+    ops.muon_step([b[0]], [b[1]], [b[2]], 0.1)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+
+
+def test_learning_rate_that_changes_in_place(dev):
+    w, g = matrices(dev, (20, 30), torch.float32, 1), matrices(dev, (20, 30), torch.float32, 2)
+    lr, got, want = torch.tensor(0.1), w.clone(), w.clone()
+    plan = ops.MuonUpdate([got], [g], [torch.zeros_like(w)])
+    m = torch.zeros_like(w)
+    for value in (0.1, 0.025):
+        lr.fill_(value)
+        plan.step(lr)
+        ops.muon_step([want], [g], [m], float(lr))
+        assert torch.equal(got, want)
+
+
 def test_muon_step_leaves_the_rest_alone(dev):
     """Rows of a wider storage: what lies between them stays."""
     store = matrices(dev, (70, 200), torch.float32, 1)

@@ -330,6 +330,11 @@ def _matrix_view(t):
     return None
 
 
+def _layout(t):
+    """Strides of the dimensions that have more than one entry."""
+    return [s for s, n in zip(t.stride(), t.shape) if n > 1]
+
+
 class MuonUpdate:
     """The step of `muon_step` on tensors that stay where they are: checked and described once, then `step(lr)` any number of times.
 
@@ -362,7 +367,7 @@ class MuonUpdate:
             if m.dtype != torch.float32 or m.device != dev or m.shape != w.shape or g.shape != w.shape:
                 raise L.WgsError("a momentum must be float32 of its param's shape on its device, got %s %s on %s and grad %s for param %s" % (
                     m.dtype, tuple(m.shape), m.device, tuple(g.shape), tuple(w.shape)))
-            if w.dim() != 2 and not (w.stride() == m.stride() == g.stride()):
+            if w.dim() != 2 and not (_layout(w) == _layout(m) == _layout(g)):
                 raise L.WgsError("a convolution weight, its gradient and its momentum must have the same layout, got strides %s %s %s" % (
                     w.stride(), g.stride(), m.stride()))
             w2, g2, m2 = _matrix_view(w), _matrix_view(g), _matrix_view(m)
@@ -395,6 +400,7 @@ class MuonUpdate:
             return
         if self._places() != self.places:
             raise L.WgsError("MuonUpdate: a tensor has been given other memory since it was described: make a new one")
+        lr = float(lr)                          # (a tensor may change in place)
         if lr != self.lr:
             decay = 1.0 - lr * self.weight_decay
             for k, f in enumerate(self.factors):
