@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from warpedganspace_amd import _lib as L
 from warpedganspace_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -92,6 +93,28 @@ def test_values_and_gradient(dev, dtype, rows, V, top, pad):
     h = torch.randn(rows, generator=gen, device=dev)
     q = torch.randn(rows, top, generator=gen, device=dev)
     check(x, labels, top, g=g, h=h, q=q)
+
+
+@pytest.mark.parametrize('V', [4097, 4098, 8193, 8195, 16385, 16390, 24577])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+def test_last_classes_of_rows_at_every_alignment(dev, dtype, V):
+    """A row whose vectors end with a workgroup's part and that has scores left behind them: their own terms belong to the last workgroup."""
+    x, labels, gen = make(dev, 24, V, dtype, V)
+    labels[:] = V - 1 - torch.arange(24, device=dev) % 3
+    with torch.no_grad():
+        x[:, -3:] += 15.0                       # alternatives too
+    g, h, q = (torch.randn(s, generator=gen, device=dev) for s in ((24,), (24,), (24, 4)))
+    check(x, labels, 4, g=g, h=h, q=q)
+    # the gradient at another place of a 16-byte block than the scores: one score at a time
+    r = ops.label_logprobs(x, labels, top=4)
+    want, = torch.autograd.grad([r.logp, r.entropy, r.top_logp], [x], [g, h, q])
+    r = ops.label_logprobs(x, labels, top=4)
+    stat = r.logp.grad_fn.saved_tensors[2]
+    out = torch.full((24, V + 3), 7.0, dtype=dtype, device=dev)
+    L.check(ops._logprobs()[2](x.data_ptr(), ops._DTYPES[dtype], 24, V, V, labels.data_ptr(), -100, stat.data_ptr(), r.entropy.data_ptr(), 4,
+                               r.top_index.data_ptr(), g.data_ptr(), h.data_ptr(), q.data_ptr(), out.data_ptr() + out.element_size(), V + 3, L.stream_id()),
+            'wgs_label_logprobs_bwd')
+    assert torch.equal(out[:, 1:V + 1], want) and (out[:, V + 1:] == 7).all() and (out[:, :1] == 7).all()
 
 
 @pytest.mark.parametrize('V', [40, 1000, 4099, 70001])

@@ -416,7 +416,8 @@ __global__ __launch_bounds__(256) void logprob_bwd_kernel(const BwdArgs a) {
     const int head0 = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(elem);
     const int head = head0 < a.V ? head0 : a.V;
     const int nvec = (a.V - head) / N, tail0 = head + nvec * N;
-    const int v0 = part * a.per, v1 = v0 + a.per < nvec ? v0 + a.per : nvec;
+    // (a row that begins off a 16-byte block can have fewer vectors than V / N: the last part is then the scores behind them)
+    const int v0 = part * a.per < nvec ? part * a.per : nvec, v1 = v0 + a.per < nvec ? v0 + a.per : nvec;
     const int from = part == 0 ? 0 : head + v0 * N, to = part == a.parts - 1 ? a.V : head + v1 * N;      // scores of this workgroup
     if ((((uintptr_t)p ^ (uintptr_t)o) & 15) == 0) {
         const uint4* pv = (const uint4*)(p + head);
