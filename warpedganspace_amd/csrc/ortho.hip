@@ -365,7 +365,7 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(const Group g, const M
 // order, B's fragments being read from LDS in the same one.  The next Gram matrix needs X with lane = row: the transposed product X^T B, from the
 // same two operands, has it, and is used and dropped block by block.  A block's fragments stay with one wave, which stores and loads them lane by
 // lane (1 KB at a time) through the caches: in registers they do not fit beside the accumulators.  The waves' partial Gram matrices are added in
-// a fixed order.  Bound by the latency of its steps and one CU's matrix cores; the many launches of the general path cost more up to these sizes.
+// a fixed order.  Bound by the latency of its steps and one CU's matrix cores; the many launches of the general path cost more where all_small says so.
 constexpr int SMALL_N = 2048, SMALL_WAVES = 8;
 struct SmallArgs { Bounds bd; float sb[MAX_STEPS]; float a, b, c; };
 __host__ __device__ __forceinline__ bool is_small(const Dims& d) { return d.m <= 64 && d.n <= SMALL_N; }
