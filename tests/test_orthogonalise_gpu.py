@@ -140,6 +140,26 @@ def test_few_rows(dev, dtype, steps, shape):
     check(ops.orthogonalise(x, steps=steps), x, steps)
 
 
+@DT
+@pytest.mark.parametrize('shape', [(3, 64, 513), (64, 1100), (16, 33, 2048), (17, 33, 2017), (32, 897), (2, 2000, 20), (2, 640, 64), (1, 1537)], ids=str)
+def test_short_matrices_with_many_columns(dev, dtype, shape):
+    x = matrices(dev, shape, dtype, 11)
+    check(ops.orthogonalise(x), x)
+
+
+@pytest.mark.parametrize('shapes', [[(64, 900), (8, 30), (200, 3)], [(1200, 20), (32, 40), (1, 1)]], ids=str)
+def test_short_steps_together(dev, shapes):
+    """A long and some short matrices in the launches of one step: workgroups without columns leave."""
+    ws, gs, ms = ([matrices(dev, s, torch.float32, 10 * k + i) for i, s in enumerate(shapes)] for k in range(3))
+    want = [step_exact(w, g, m, 0.05, 0.9, True, 0.1, 0.5) for w, g, m in zip(ws, gs, ms)]
+    ops.muon_step(ws, gs, ms, 0.05, momentum=0.9, nesterov=True, weight_decay=0.1, grad_scale=0.5)
+    for w, m, (w1, m1, u, f) in zip(ws, ms, want):
+        assert float((m.double() - m1).abs().max()) <= 3 * 2.0 ** -24 * float(m1.abs().max() + 5)
+        model = (noisy(u.float(), phases_of(torch.float32, 5)) - exact(u.float())).square().sum().sqrt()
+        allowed = 0.05 * f * (12 * model + 2.0 ** -20 * exact(u).square().sum().sqrt()) + 1.1 * 2.0 ** -24 * w1.square().sum().sqrt()
+        assert float((w.double() - w1).square().sum().sqrt()) <= float(allowed)
+
+
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=['bf16', 'f16'])
 @pytest.mark.parametrize('shapes', [[(33, 4100), (2, 128, 140), (1, 2500), (90, 3)], [(1, 4100), (31, 2100), (2, 64, 2049)], [(128, 300), (129, 300)]], ids=str)
 def test_few_rows_together(dev, dtype, shapes):

@@ -367,25 +367,33 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(const Group g, const M
 // lane (1 KB at a time) through the caches: in registers they do not fit beside the accumulators.  The waves' partial Gram matrices are added in
 // a fixed order.  Bound by the latency of its steps and one CU's matrix cores; the many launches of the general path cost more where all_small says so.
 constexpr int SMALL_N = 2048, SMALL_WAVES = 8;
-struct SmallArgs { Bounds bd; float sb[MAX_STEPS]; float a, b, c; };
+// With many columns it is a launch a step instead, PARTS_WAVES blocks a workgroup (WHOLE = false; the norm comes from its kernel): a workgroup adds the
+// partial Gram matrices of its matrix's workgroups, in order, forms B, applies it to its blocks and leaves its part of the next Gram matrix.
+constexpr int PARTS_WAVES = 4;
+struct SmallArgs { Bounds bd; float sb[MAX_STEPS]; float a, b, c; int t, parts; };      // WHOLE = false: the step (-1: the operands), most workgroups a matrix
 __host__ __device__ __forceinline__ bool is_small(const Dims& d) { return d.m <= 64 && d.n <= SMALL_N; }
-__host__ __device__ __forceinline__ int64_t small_bytes(const Dims& d) { return 64 * (int64_t)d.np * 4; }
-template <int MT>
-__global__ __launch_bounds__(64 * SMALL_WAVES, 1) void ortho_small_kernel(const Group g, const Momentum mo, const SmallArgs ar) {
-    constexpr int W = SMALL_WAVES, TRI = MT * (MT + 1) / 2, LD = 32 * MT + 8, TURNS = 16 * MT, U = 16;
+__host__ __device__ __forceinline__ int64_t small_parts(const Dims& d) { return (d.np / 32 + PARTS_WAVES - 1) / PARTS_WAVES; }
+__host__ __device__ __forceinline__ int64_t small_bytes(const Dims& d) { return 64 * (int64_t)d.np * 4 + 2 * small_parts(d) * (3 * 1024 * 4); }      // X, two sets of partial Gram matrices
+template <int MT, bool WHOLE>
+__global__ __launch_bounds__(64 * (WHOLE ? SMALL_WAVES : PARTS_WAVES), 1) void ortho_small_kernel(const Group g, const Momentum mo, const SmallArgs ar) {
+    constexpr int W = WHOLE ? SMALL_WAVES : PARTS_WAVES, TRI = MT * (MT + 1) / 2, LD = 32 * MT + 8, TURNS = 16 * MT, U = 16;
     __shared__ float part[W][TRI][32][33];
     __shared__ __attribute__((aligned(16))) _Float16 sa[2][32 * MT][LD], sbm[2][32 * MT][LD];
     __shared__ double rs[W];
     __shared__ float rm[W];
     __shared__ float info[INFO];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, lh = lane >> 5;
-    const Mat& mat = g.mat[entry_of(g, blockIdx.x)];
-    const int b = blockIdx.x - mat.first;
+    const int inst = WHOLE ? blockIdx.x : blockIdx.x / (unsigned)ar.parts, pw = WHOLE ? 0 : blockIdx.x % (unsigned)ar.parts;
+    const Mat& mat = g.mat[entry_of(g, inst)];
+    const int b = inst - mat.first;
     const Dims d = dims_of(mat.M, mat.N);
+    const int parts = WHOLE ? 1 : (int)small_parts(d);
+    if (pw >= parts) return;
     const bool wide = mat.M <= mat.N;
     const int64_t off = b * mat.in_bs, moff = (int64_t)b * mat.M * mat.N, ob = b * mat.out_bs;
+    float* const sums = (float*)(g.ws + mat.ws + b * small_bytes(d) + 64 * (int64_t)d.np * 4);       // [2][parts][TRI][1024]
     float* tr = &part[wave][0][0][0];          // a wave's own [32 MT rows i][33]
-    const int blocks = d.np / 32, active = blocks < W ? blocks : W;
+    const int blocks = d.np / 32, k0 = pw * W + wave, kstep = parts * W, active = blocks - pw * W < W ? blocks - pw * W : W;
     frag* const frags = (frag*)(g.ws + mat.ws + b * small_bytes(d)) + lane;      // block k: [tile][half][hi, lo][64 lanes]
     auto at = [&](int k, int t, int ks, int pl) { return frags + (((int64_t)k * MT + t) * 4 + ks * 2 + pl) * 64; };
     auto split = [&](const float* v, frag& fh, frag& fl) {
@@ -443,24 +451,6 @@ __global__ __launch_bounds__(64 * SMALL_WAVES, 1) void ortho_small_kernel(const 
             }
         });
     };
-    double ss = 0.0;
-    float amax = 0.f;
-#pragma unroll 1
-    for (int k = wave; k < blocks; k += W)
-        input(true, k, 1.f, [&](int, float v) {
-            ss = __builtin_fma((double)v, (double)v, ss);
-            amax = fmaxf(amax, fabsf(v));
-        });
-    ss = wave_sum_d(ss);
-    amax = wave_max(amax);
-    if (lane == 0) { rs[wave] = ss; rm[wave] = amax; }
-    __syncthreads();
-    ss = 0.0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) { ss += rs[w]; amax = fmaxf(amax, rm[w]); }
-    const float mult = scale_of(ss, amax);
-    if (tid == 0) write_info(info, ss, amax, mult, d.n, ar.bd);
-
     f32x16 gr[TRI];
     auto gram = [&](const frag (&ih)[MT][2], const frag (&il)[MT][2]) __attribute__((always_inline)) {       // adds one block: lane = row i, 8 columns a fragment
 #pragma unroll
@@ -479,10 +469,51 @@ __global__ __launch_bounds__(64 * SMALL_WAVES, 1) void ortho_small_kernel(const 
 #pragma unroll
             for (int q = 0; q < 16; ++q) gr[t][q] = 0.f;
     };
+    auto leave = [&](int l31, int lh) __attribute__((always_inline)) {          // a wave's part of the Gram matrix into the LDS
+        if (wave < active)
+#pragma unroll
+            for (int k = 0; k < TRI; ++k)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) part[wave][k][8 * (q >> 2) + 4 * lh + (q & 3)][l31] = gr[k][q];
+        __syncthreads();
+    };
+    auto publish = [&](int t) __attribute__((always_inline)) {                  // WHOLE = false: the workgroup's part, for step t
+        leave(l31, lh);
+        float* o = sums + ((t & 1) * parts + pw) * (TRI * 1024);
+        for (int e = tid; e < TRI * 1024; e += 64 * W) {
+            const int k = e >> 10, r = (e >> 5) & 31, c = e & 31;
+            float v = part[0][k][r][c];
+            for (int w = 1; w < active; ++w) v += part[w][k][r][c];
+            o[e] = v;
+        }
+    };
+    if (WHOLE || ar.t < 0) {
+    double ss = 0.0;
+    float amax = 0.f;
+    if (!WHOLE) {
+        const Part* p = parts_of(g, inst);
+        if (tid < g.stat_blocks) { ss = p[tid].ss; amax = p[tid].amax; }
+    } else
+#pragma unroll 1
+    for (int k = wave; k < blocks; k += W)
+        input(true, k, 1.f, [&](int, float v) {
+            ss = __builtin_fma((double)v, (double)v, ss);
+            amax = fmaxf(amax, fabsf(v));
+        });
+    ss = wave_sum_d(ss);
+    amax = wave_max(amax);
+    if (lane == 0) { rs[wave] = ss; rm[wave] = amax; }
+    __syncthreads();
+    ss = 0.0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) { ss += rs[w]; amax = fmaxf(amax, rm[w]); }
+    const float mult = scale_of(ss, amax);
+    if (tid == 0 && pw == 0) write_info(WHOLE ? info : info_of(g, inst), ss, amax, mult, d.n, ar.bd);
+
     // the operands, through LDS: lane = column to stay, lane = row for the first Gram matrix
     clear();
 #pragma unroll 1
-    for (int k = wave; k < blocks; k += W) {
+    for (int k = k0; k < blocks; k += kstep) {
         asm volatile("" ::: "memory");
         input(false, k, mult, [&](int i, float v) { tr[i] = v; });
         asm volatile("" ::: "memory");
@@ -505,25 +536,43 @@ __global__ __launch_bounds__(64 * SMALL_WAVES, 1) void ortho_small_kernel(const 
         }
         gram(ih, il);
     }
+    if (!WHOLE) { publish(0); return; }
+    }
+    frag nh[MT][2], nl[MT][2];               // the next block's fragments
+    auto load = [&](int k) {
+#pragma unroll
+        for (int u = 0; u < MT; ++u)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) { nh[u][ks] = *at(k, u, ks, 0); nl[u][ks] = *at(k, u, ks, 1); }
+    };
+    if (!WHOLE && k0 < blocks) load(k0);
+    const float* const inf = WHOLE ? info : info_of(g, inst);
 #pragma unroll 1
-    for (int t = 0; t < ar.bd.steps; ++t) {
+    for (int t = WHOLE ? 0 : ar.t; t < (WHOLE ? ar.bd.steps : ar.t + 1); ++t) {
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid) :: "memory");       // (nor the LDS addresses from step to step)
         const int lane = tid & 63, l31 = lane & 31, lh = lane >> 5;
-        if (wave < active)
+        constexpr int EACH = TRI * 1024 / (64 * W);
+        float sum[EACH];
+        if (WHOLE) leave(l31, lh);
+        else {
+            const float* src = sums + (t & 1) * parts * (TRI * 1024) + tid;
 #pragma unroll
-            for (int k = 0; k < TRI; ++k)
+            for (int it = 0; it < EACH; ++it) sum[it] = src[it * 64 * W];
+#pragma unroll 2
+            for (int w = 1; w < parts; ++w)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) part[wave][k][8 * (q >> 2) + 4 * lh + (q & 3)][l31] = gr[k][q];
-        __syncthreads();
-        const float fx = t == 0 ? info[0] : 1.f / info[I_SX + t], sA = info[I_SA + t], ga = fx * fx * sA;
+                for (int it = 0; it < EACH; ++it) sum[it] += src[w * (TRI * 1024) + it * 64 * W];
+        }
+        const float fx = t == 0 ? inf[0] : 1.f / inf[I_SX + t], sA = inf[I_SA + t], ga = fx * fx * sA;
 #pragma unroll
-        for (int it = 0; it < TRI * 1024 / (64 * W); ++it) {
+        for (int it = 0; it < EACH; ++it) {
             const int e = it * 64 * W + tid, k = e >> 10, r = (e >> 5) & 31, c = e & 31;
             const int p = k == 0 ? 0 : 1, q = k == 2 ? 1 : 0;
             if (p == q && r < c) continue;
-            float v = part[0][k][r][c];
-            for (int w = 1; w < active; ++w) v += part[w][k][r][c];
+            float v = WHOLE ? part[0][k][r][c] : sum[it];
+            if (WHOLE)
+                for (int w = 1; w < active; ++w) v += part[w][k][r][c];
             _Float16 h, l;
             split_pair(v * ga, h, l);
             sa[0][32 * p + r][32 * q + c] = h; sa[1][32 * p + r][32 * q + c] = l;
@@ -560,24 +609,17 @@ __global__ __launch_bounds__(64 * SMALL_WAVES, 1) void ortho_small_kernel(const 
         }
         __syncthreads();
         const bool last = t + 1 == ar.bd.steps;
-        const float fo = last ? fx / ar.sb[t] : fx * info[I_SX + t + 1] / ar.sb[t];
+        const float fo = last ? fx / ar.sb[t] : fx * inf[I_SX + t + 1] / ar.sb[t];
         clear();
-        frag nh[MT][2], nl[MT][2];               // the next block's fragments
-        auto load = [&](int k) {
-#pragma unroll
-            for (int u = 0; u < MT; ++u)
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) { nh[u][ks] = *at(k, u, ks, 0); nl[u][ks] = *at(k, u, ks, 1); }
-        };
-        if (wave < blocks) load(wave);
+        if (WHOLE && k0 < blocks) load(k0);
 #pragma unroll 1
-        for (int k = wave; k < blocks; k += W) {
+        for (int k = k0; k < blocks; k += kstep) {
             frag vh[MT][2], vl[MT][2];
 #pragma unroll
             for (int u = 0; u < MT; ++u)
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) { vh[u][ks] = nh[u][ks]; vl[u][ks] = nl[u][ks]; }
-            load(k + W < blocks ? k + W : k);
+            if (WHOLE) load(k + W < blocks ? k + W : k);
             // B X (lane = column) and, from the same operands in the other order, X^T B (lane = row)
             f32x16 dd[MT], de[MT];
 #pragma unroll
@@ -660,6 +702,7 @@ __global__ __launch_bounds__(64 * SMALL_WAVES, 1) void ortho_small_kernel(const 
                 }
             }
         }
+        if (!WHOLE && !last) publish(t + 1);
     }
 }
 
@@ -1461,33 +1504,53 @@ int gemm(const Group& g, const Jobs& js, hipStream_t st) {
 }
 
 template <int DT, bool STEP>
-void launch_prepare(const Group& g, const Momentum& mo, const Bounds& bd, hipStream_t st) {
+void launch_norm(const Group& g, const Momentum& mo, hipStream_t st) {
     WGS_LAUNCH((ortho_norm_kernel<DT, STEP>), dim3((unsigned)(g.instances * g.stat_blocks)), dim3(512), 0, st, g, mo);
+}
+template <int DT, bool STEP>
+void launch_prepare(const Group& g, const Momentum& mo, const Bounds& bd, hipStream_t st) {
+    launch_norm<DT, STEP>(g, mo, st);
     int64_t tiles = 0;
     for (int i = 0; i < g.count; ++i) tiles += (int64_t)g.mat[i].batch * ((up(g.mat[i].M, BK) + 63) / 64) * ((up(g.mat[i].N, BK) + 63) / 64);
     WGS_LAUNCH((ortho_split_kernel<DT, STEP>), dim3((unsigned)tiles), dim3(256), 0, st, g, mo, bd, (int)tiles);
 }
 
 bool all_small(const Group& g, const Plan& p, int steps) {
-    // One workgroup a matrix takes some (5 + 0.022 n) us a step at m = 64, the general path's many workgroups are done sooner with long rows.  Single
-    // iterations: where there are few matrices of over 1024 columns (64 x 2000 fp32: 245 against some 160 us).  Joined ones, with the chain kernel: m > 32
-    // from some 640 phases / steps columns (one of 64 x 64 bf16 40 against 45 us, 64 x 256 61 / 47, 64 x 1000 142 / 51, 512 of them 396 / 196; fp16, two
-    // phases: 64 x 64 40 / 60, 64 x 256 61 / 64, 64 x 576 98 / 67), m <= 32 like single ones (32 x 256 bf16 27 / 47, 32 x 2000 95 / 55).
+    // Single iterations: always.  Joined ones with m > 32 go on through the chain kernel, whose launches outweigh its work up to some 1000 phases / steps
+    // columns (64 x 64 bf16 35 us here, 45 there, 64 x 256 48 / 47, 64 x 1000 113 / 51; fp16, two phases: 64 x 256 48 / 64, 64 x 576 80 / 67).
     const bool joined = p.phases < steps;
     for (int i = 0; i < g.count; ++i) {
         const Dims d = dims_of(g.mat[i].M, g.mat[i].N);
-        if (!is_small(d)) return false;
-        if (joined && d.m > 32 && d.n * steps > 640 * p.phases) return false;
-        if ((joined || d.m > 32) && d.n > 1024 && g.instances < 32) return false;
+        if (!is_small(d) || (joined && d.m > 32 && d.n * steps > 1000 * p.phases)) return false;
     }
     return true;
 }
-void launch_small(const Group& g, const Momentum& mo, const SmallArgs& ar, hipStream_t st) {
-    int m = 0;
-    for (int i = 0; i < g.count; ++i) { const int x = dims_of(g.mat[i].M, g.mat[i].N).m; if (x > m) m = x; }
-    const dim3 gr((unsigned)g.instances), bl(64 * SMALL_WAVES);
-    if (m <= 32) WGS_LAUNCH(ortho_small_kernel<1>, gr, bl, 0, st, g, mo, ar);
-    else WGS_LAUNCH(ortho_small_kernel<2>, gr, bl, 0, st, g, mo, ar);
+void launch_small(const Group& g, const Momentum& mo, SmallArgs ar, hipStream_t st) {
+    int m = 0, n = 0;
+    ar.parts = 1;
+    for (int i = 0; i < g.count; ++i) {
+        const Dims d = dims_of(g.mat[i].M, g.mat[i].N);
+        if (d.m > m) m = d.m;
+        if (d.n > n) n = d.n;
+        if (small_parts(d) > ar.parts) ar.parts = (int)small_parts(d);
+    }
+    // A step of its own launch costs some 10 us whatever n is, in one launch some 3 + n / 50 (m = 64), n / 120 (m = 32), but the other matrices wait for a
+    // CU: one of 64 x 576 fp32 80 against 73 us, 64 x 1000 113 / 79, 32 x 1000 57 / 51, 32 x 2000 97 / 57; 64 of 64 x 1000 (512 workgroups) 116 / 187.
+    if (n <= (m > 32 ? 512 : 896) || (int64_t)g.instances * ar.parts > 256) {
+        const dim3 gr((unsigned)g.instances), bl(64 * SMALL_WAVES);
+        if (m <= 32) WGS_LAUNCH((ortho_small_kernel<1, true>), gr, bl, 0, st, g, mo, ar);
+        else WGS_LAUNCH((ortho_small_kernel<2, true>), gr, bl, 0, st, g, mo, ar);
+        return;
+    }
+    const bool step = g.step;
+    if (g.dtype == WGS_F32) { if (step) launch_norm<WGS_F32, true>(g, mo, st); else launch_norm<WGS_F32, false>(g, mo, st); }
+    else if (g.dtype == WGS_BF16) { if (step) launch_norm<WGS_BF16, true>(g, mo, st); else launch_norm<WGS_BF16, false>(g, mo, st); }
+    else { if (step) launch_norm<WGS_F16, true>(g, mo, st); else launch_norm<WGS_F16, false>(g, mo, st); }
+    const dim3 gr((unsigned)(g.instances * ar.parts)), bl(64 * PARTS_WAVES);
+    for (ar.t = -1; ar.t < ar.bd.steps; ++ar.t) {
+        if (m <= 32) WGS_LAUNCH((ortho_small_kernel<1, false>), gr, bl, 0, st, g, mo, ar);
+        else WGS_LAUNCH((ortho_small_kernel<2, false>), gr, bl, 0, st, g, mo, ar);
+    }
 }
 
 int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step, const Momentum& mo, int steps, double a, double b, double c, float eps, void* ws,
