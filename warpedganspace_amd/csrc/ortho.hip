@@ -359,7 +359,7 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(const Group g, const M
     }
 }
 
-// ---- small matrices: everything in one launch -------------------------------------------------------------------------------------------------
+// ---- small matrices: everything in one launch, or a launch a step -------------------------------------------------------------------------------------------------
 // m <= 32 MT <= 64, n <= SMALL_N: one workgroup a matrix, the m x m matrices in LDS.  X lies in blocks of 32 columns as the operand "lane = column j,
 // 8 rows i": the product's own result layout (lane = column, rows 8 q + 4 half + 0..3) is an operand again once the sum's index is taken in that
 // order, B's fragments being read from LDS in the same one.  The next Gram matrix needs X with lane = row: the transposed product X^T B, from the
