@@ -367,16 +367,16 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(const Group g, const M
 // lane (1 KB at a time) through the caches: in registers they do not fit beside the accumulators.  The waves' partial Gram matrices are added in
 // a fixed order.  Bound by the latency of its steps and one CU's matrix cores; the many launches of the general path cost more where all_small says so.
 constexpr int SMALL_N = 2048, SMALL_WAVES = 8;
-// With many columns it is a launch a step instead, PARTS_WAVES blocks a workgroup (WHOLE = false; the norm comes from its kernel): a workgroup adds the
-// partial Gram matrices of its matrix's workgroups, in order, forms B, applies it to its blocks and leaves its part of the next Gram matrix.
-constexpr int PARTS_WAVES = 4;
+// With many columns it is a launch a step instead, a block a wave (WHOLE = false; the norm comes from its kernel): a workgroup adds the partial Gram
+// matrices of its matrix's workgroups, in order, forms B, applies it to its blocks and leaves its part of the next Gram matrix.  (Workgroups of four
+// and two waves have more parts to add and fewer threads to do it: 4 x 64 x 576 fp32 68 us with eight, 74, 85.)
 struct SmallArgs { Bounds bd; float sb[MAX_STEPS]; float a, b, c; int t, parts; };      // WHOLE = false: the step (-1: the operands), most workgroups a matrix
 __host__ __device__ __forceinline__ bool is_small(const Dims& d) { return d.m <= 64 && d.n <= SMALL_N; }
-__host__ __device__ __forceinline__ int64_t small_parts(const Dims& d) { return (d.np / 32 + PARTS_WAVES - 1) / PARTS_WAVES; }
+__host__ __device__ __forceinline__ int64_t small_parts(const Dims& d) { return (d.np / 32 + SMALL_WAVES - 1) / SMALL_WAVES; }
 __host__ __device__ __forceinline__ int64_t small_bytes(const Dims& d) { return 64 * (int64_t)d.np * 4 + 2 * small_parts(d) * (3 * 1024 * 4); }      // X, two sets of partial Gram matrices
 template <int MT, bool WHOLE>
-__global__ __launch_bounds__(64 * (WHOLE ? SMALL_WAVES : PARTS_WAVES), 1) void ortho_small_kernel(const Group g, const Momentum mo, const SmallArgs ar) {
-    constexpr int W = WHOLE ? SMALL_WAVES : PARTS_WAVES, TRI = MT * (MT + 1) / 2, LD = 32 * MT + 8, TURNS = 16 * MT, U = 16;
+__global__ __launch_bounds__(64 * SMALL_WAVES, 1) void ortho_small_kernel(const Group g, const Momentum mo, const SmallArgs ar) {
+    constexpr int W = SMALL_WAVES, TRI = MT * (MT + 1) / 2, LD = 32 * MT + 8, TURNS = 16 * MT, U = 16;
     __shared__ float part[W][TRI][32][33];
     __shared__ __attribute__((aligned(16))) _Float16 sa[2][32 * MT][LD], sbm[2][32 * MT][LD];
     __shared__ double rs[W];
@@ -1534,9 +1534,10 @@ void launch_small(const Group& g, const Momentum& mo, SmallArgs ar, hipStream_t 
         if (d.n > n) n = d.n;
         if (small_parts(d) > ar.parts) ar.parts = (int)small_parts(d);
     }
-    // A step of its own launch costs some 10 us whatever n is, in one launch some 3 + n / 50 (m = 64), n / 120 (m = 32), but the other matrices wait for a
-    // CU: one of 64 x 576 fp32 80 against 73 us, 64 x 1000 113 / 79, 32 x 1000 57 / 51, 32 x 2000 97 / 57; 64 of 64 x 1000 (512 workgroups) 116 / 187.
-    if (n <= (m > 32 ? 512 : 896) || (int64_t)g.instances * ar.parts > 256) {
+    // A step of its own launch costs some 9 us (m = 64) or 6 (m = 32) almost whatever n is, in one launch it grows with the blocks of a wave; but a workgroup
+    // takes a CU.  One matrix in fp32: 64 x 384 (two blocks a wave) 62 against some 65 us, 64 x 576 80 / 67, 64 x 1000 113 / 69, 32 x 640 (three blocks) 43 / 42,
+    // 32 x 1000 57 / 45, 32 x 2000 97 / 49; 64 of 64 x 1000 116 / 92.
+    if (n <= 32 * SMALL_WAVES * (m > 32 ? 2 : 3) || (int64_t)g.instances * ar.parts > 256) {
         const dim3 gr((unsigned)g.instances), bl(64 * SMALL_WAVES);
         if (m <= 32) WGS_LAUNCH((ortho_small_kernel<1, true>), gr, bl, 0, st, g, mo, ar);
         else WGS_LAUNCH((ortho_small_kernel<2, true>), gr, bl, 0, st, g, mo, ar);
@@ -1546,7 +1547,7 @@ void launch_small(const Group& g, const Momentum& mo, SmallArgs ar, hipStream_t 
     if (g.dtype == WGS_F32) { if (step) launch_norm<WGS_F32, true>(g, mo, st); else launch_norm<WGS_F32, false>(g, mo, st); }
     else if (g.dtype == WGS_BF16) { if (step) launch_norm<WGS_BF16, true>(g, mo, st); else launch_norm<WGS_BF16, false>(g, mo, st); }
     else { if (step) launch_norm<WGS_F16, true>(g, mo, st); else launch_norm<WGS_F16, false>(g, mo, st); }
-    const dim3 gr((unsigned)(g.instances * ar.parts)), bl(64 * PARTS_WAVES);
+    const dim3 gr((unsigned)(g.instances * ar.parts)), bl(64 * SMALL_WAVES);
     for (ar.t = -1; ar.t < ar.bd.steps; ++ar.t) {
         if (m <= 32) WGS_LAUNCH((ortho_small_kernel<1, false>), gr, bl, 0, st, g, mo, ar);
         else WGS_LAUNCH((ortho_small_kernel<2, false>), gr, bl, 0, st, g, mo, ar);
