@@ -7,8 +7,8 @@
 // and all of them are symmetric: their products compute the tiles on and under the diagonal and write each twice.
 //
 // Arithmetic.  The iteration multiplies small singular values by a = 3.44 each time (A's eigenvalues by a^2), and the noise of the products with
-// them, so the products keep fp32's precision: an operand is an fp16 pair hi + lo = value * 2^s (22 bits), a product lo*hi + hi*lo + hi*hi on
-// the 16-bit matrix cores with fp32 accumulation — 3 / 2 500 of a TFLOP instead of 1 / 157 on the fp32 ones.  Exponents: X from its largest
+// them, so the products keep about fp32's precision (plan_of has the measured distances): an operand is an fp16 pair hi + lo = value * 2^s (22 bits),
+// a product lo*hi + hi*lo + hi*hi on the 16-bit matrix cores with fp32 accumulation — 3 / 2 500 of a TFLOP instead of 1 / 157 on the fp32 ones.  Exponents: X from its largest
 // entry; A_t, X_t from bounds on their entries (|A_ij| <= max_i |x_i|^2, times the largest |a + b l + c l^2|^2 on the interval that the
 // eigenvalues can reach, iteration by iteration); B, Q from the same polynomial's maximum.  16-bit inputs are their own hi part (one product in
 // the first Gram matrix, two in its phase's Q X).  Norms are summed in fp64.
@@ -1325,12 +1325,31 @@ __global__ __launch_bounds__(512, 1) void ortho_chain_kernel(const Group g, cons
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------
 struct Plan { int phases, len[MAX_STEPS]; int planes, npx, nt, ns; };
 // Iterations of a phase.  Longer phases leave out products with the n columns, but A_t then carries its own rounding through a^2 a step instead
-// of being formed anew from X_t: measured on spectra from flat to a single spike, one phase of five is within 5e-4 of the exact factor, (3, 2)
-// within 5e-5, single iterations within the 32-bit iteration's own 3e-5 (1e-6 .. 1e-5 for noise-dominated matrices).  So: what the result's
-// type can hold.
-Plan plan_of(int dtype, bool step, int steps) {
+// of being formed anew from X_t.  Distance from the exact factor before the result is rounded (relative, Frobenius; 48 x 600 .. 2048 x 2048, fp32
+// in and out), against the iteration on 32-bit library products:
+//                                        32-bit    single    (3, 2)    five
+//   noise, rows of uneven size           5e-6      2e-6      6e-6      9e-6
+//   one direction in noise of 0.1        5e-6      2e-6      5e-6      3e-4
+//   ... of 0.01                          5e-5      2e-5      2e-5      6e-4
+//   ... of 0.001, 0.0001                 4e-4      1.3e-4    1.3e-4    6e-4
+//   eight directions in noise of 0.01    6e-5      4e-5      3e-5      2e-4
+//   a third of the rank; 5 decades       9e-6      1.3e-5    8e-6      3e-4
+// Single iterations are at most 1.4 times as far as 32-bit products (mostly nearer: the sums have fewer roundings), (3, 2) as good as they.
+// Five are not: they put a bf16 result up to 11 % further from the exact factor than its rounding does, and save 1.4 ms of 6.1 at 4096 x 16384
+// (single iterations: 10.3), 30 us of 136 at 64 of 128 x 512.  So bf16 takes five, fp16 three, fp32 one, where the caller names no number;
+// nearly square matrices of over 128 rows, whose products with X cost no more than those they replace, one whatever the type (bf16 singles / (3, 2) /
+// five: 1024^2 217 / 251 / 245 us, 2048^2 874 / 977 / 958, 4096^2 3.45 / 3.69 / 3.75 ms; but 4096 x 4608 4.47 / 4.06 / 3.89).
+Plan plan_of(int dtype, bool step, int steps, const wgs_matrix* mats, int count) {
     Plan p;
-    const int most = dtype == WGS_BF16 ? 5 : dtype == WGS_F16 ? 3 : 1;
+    int most = count ? mats[0].joined : 1;
+    if (!most) {
+        most = 1;
+        if (dtype != WGS_F32)
+            for (int i = 0; i < count; ++i) {
+                const Dims d = dims_of(mats[i].rows, mats[i].cols);
+                if (mats[i].batch && (d.m <= 128 || d.n - d.m > d.m / 16)) most = dtype == WGS_BF16 ? 5 : 3;
+            }
+    }
     p.phases = (steps + most - 1) / most;
     int longest = 0;
     for (int i = 0, left = steps; i < p.phases; ++i) {
@@ -1403,6 +1422,7 @@ const char* check_mats(const wgs_matrix* mats, int count, int dtype, bool step, 
             return "bad sizes (rows, cols >= 1, fewer than 2^29 elements with the smaller side's padding to 32)";
         if (w.in_row_stride < w.cols || w.out_row_stride < w.cols || w.in_row_stride >= (1LL << 31) || w.out_row_stride >= (1LL << 31)) return "row strides must be at least cols";
         if (w.batch > 1 && (w.in_batch_stride < 0 || w.out_batch_stride < (int64_t)(w.rows - 1) * w.out_row_stride + w.cols)) return "batch strides overlap";
+        if (w.joined < 0 || w.joined > MAX_STEPS || w.joined != mats[0].joined) return "joined must be 0 .. 16 and the same in all matrices of a call";
         if (w.batch > (1 << 20)) return "batch must be at most 2^20";
         if (w.batch && (!w.in || !w.out || (step && !w.momentum))) return "null pointer";
         const uintptr_t am = dtype == WGS_F32 ? 3 : 1;
@@ -1412,7 +1432,7 @@ const char* check_mats(const wgs_matrix* mats, int count, int dtype, bool step, 
 }
 
 int64_t workspace(const wgs_matrix* mats, int count, int dtype, bool step, int steps) {
-    const Plan p = plan_of(dtype, step, steps);
+    const Plan p = plan_of(dtype, step, steps, mats, count);
     Cursor c;
     Group g;
     g.dtype = dtype;
@@ -1574,7 +1594,7 @@ int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step
         WGS_CHECK_ARG(next < 1e6 && q[t] < 1e6 && q[t] > 0, "%s: the iteration with these coefficients does not stay bounded", who);
         grow = fmin(grow * q[t] * q[t], 1e30); cap = next;
     }
-    const Plan p = plan_of(dtype, step, steps);
+    const Plan p = plan_of(dtype, step, steps, mats, count);
     Cursor cur;
     Group g;
     g.dtype = dtype; g.step = step; g.npx = p.npx; g.nt = p.nt; g.ns = p.ns; g.ws = (unsigned char*)ws;
