@@ -1,0 +1,32 @@
+"""The momentum step as a PyTorch user meets it: graphs that hold its tensors, tensors that overlap, gradients that are made anew."""
+import pytest
+import torch
+
+from warpedganspace_amd import _lib as L
+from warpedganspace_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_graph_that_saved_a_weight_before_the_step_is_refused(dev):
+    w = torch.randn(12, 20, device=dev, requires_grad=True)
+    g, m = torch.randn(12, 20, device=dev), torch.zeros(12, 20, device=dev)
+    before = w._version, m._version, g._version
+    loss, product = w.square().sum(), (m * w).sum()
+    ops.muon_step([w], [g], [m], 0.1)
+    assert w._version > before[0] and m._version > before[1] and g._version == before[2]
+    for late in (loss, product):
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            late.backward()
+    w.square().sum().backward()                # of the new weight
+    assert torch.equal(w.grad, 2 * w.detach())
+    plan = ops.MuonUpdate([w], [g], [m])
+    loss = w.square().sum()
+    plan.step(0.1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    with torch.inference_mode():               # tensors without a counter are stepped as ever
+        t = [torch.randn(4, 6, device=dev) for _ in range(2)] + [torch.zeros(4, 6, device=dev)]
+        old = t[0].clone()
+        ops.muon_step([t[0]], [t[1]], [t[2]], 0.1)
+        assert not torch.equal(t[0], old)

@@ -426,6 +426,8 @@ class MuonUpdate:
             ws = torch.empty(self.need, dtype=torch.uint8, device=self.device)
             L.check(L.lib().wgs_muon_step(self.mats, self.n, self.code, self.args[0], self.args[1], L.c_float(self.grad_scale), self.steps, *self.rest,
                                           L.rawptr(ws), L.c_int64(self.need), L.stream()), 'wgs_muon_step')
+        # (a graph that saved a weight before the step may not use it after)
+        torch.autograd.graph.increment_version(self.tensors[0] + self.tensors[2])
 
 
 _STEP_DECAY, _STEP_DECAY_AT = struct.Struct('=2f'), struct.calcsize('=3Q4q3i')
