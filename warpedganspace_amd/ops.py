@@ -396,9 +396,10 @@ class MuonUpdate:
                 if (N > 1 and t.stride(1) != 1) or (M > 1 and t.stride(0) < N):
                     raise L.WgsError("%s: the elements of a row must be adjacent, got strides %s" % (what, t.stride()))
             gr, wr = (g2.stride(0), w2.stride(0)) if M > 1 else (N, N)
-            spans.append((m2.data_ptr(), m2.data_ptr() + 4 * M * N, True, True))
-            spans.append((w2.data_ptr(), w2.data_ptr() + w2.element_size() * ((M - 1) * wr + N), wr == N, True))
-            spans.append((g2.data_ptr(), g2.data_ptr() + g2.element_size() * ((M - 1) * gr + N), gr == N, False))
+            size = w2.element_size()
+            spans.append((m2.data_ptr(), 1, 4 * M * N, 4 * M * N, True))
+            for t, r, written in ((w2, wr, True), (g2, gr, False)):
+                spans.append((t.data_ptr(), 1, size * M * N, size * M * N, written) if r == N else (t.data_ptr(), M, size * N, size * r, written))
             self.factors.append(max(1.0, M / N) ** 0.5 if scale is None else 0.2 * max(M, N) ** 0.5 if scale == 'rms' else float(scale))
             _MATRIX.pack_into(self.mats, k * _MATRIX.size, g2.data_ptr(), w2.data_ptr(), m2.data_ptr(), 0, 0, gr, wr, M, N, 1, 0.0, 1.0, joined)
         _check_apart(spans)
@@ -434,16 +435,36 @@ _STEP_DECAY, _STEP_DECAY_AT = struct.Struct('=2f'), struct.calcsize('=3Q4q3i')
 
 
 def _check_apart(spans):
-    """What a step writes may overlap neither what else it writes nor the gradients: spans (start, end, dense, written) in bytes.  A span that
-    begins inside a dense one overlaps it; inside a strided one it may lie between the rows."""
-    end = {True: 0, False: 0}                   # of the dense spans so far, written and read
-    start = {True: -1, False: -1}
-    for a, b, dense, written in sorted(spans):
-        if a < end[True] or a == start[True] or (written and (a < end[False] or a == start[False])):
-            raise L.WgsError("muon_step: a param or momentum is given twice, or overlaps another tensor of the call")
-        start[written] = a
-        if dense:
-            end[written] = max(end[written], b)
+    """What a step writes may overlap neither what else it writes nor the gradients: spans (start, rows, bytes of a row, bytes between rows,
+    written).  Rows of one may lie between the rows of another."""
+    live = []                                   # spans that reach behind the start of the one at hand
+    for span in sorted((a, a + (rows - 1) * step + size, rows, size, step, written) for a, rows, size, step, written in spans):
+        live = [s for s in live if s[1] > span[0]]
+        for other in live:
+            if (span[5] or other[5]) and _rows_meet(other, span):
+                raise L.WgsError("muon_step: a param or momentum is given twice, or overlaps another tensor of the call")
+        live.append(span)
+
+
+def _rows_meet(p, q):
+    """Whether a row of p and one of q share a byte; (start, end, rows, bytes of a row, bytes between rows, ..), ascending rows apart from each other."""
+    if p[2] > q[2]:
+        p, q = q, p
+    a, _, rows, size, step = p[:5]
+    b, end, _, qsize, qstep = q[:5]
+    if step == qstep and rows > 1:
+        # row i of p against row i + k of q: the same for all i, so the two k around the first row's place decide, where such rows exist
+        k = (a - b) // step
+        return any(max(0, -n) < min(rows, q[2] - n) and b + n * step < a + size and a < b + n * step + qsize for n in (k, k + 1))
+    for i in range(max(0, -((a + size - 1 - b) // step)), rows):
+        first = a + i * step
+        if first >= end:
+            return False
+        if first + size > b:
+            last = min(q[2] - 1, (first + size - 1 - b) // qstep)       # q's last row that begins before this one ends: the others end earlier
+            if b + last * qstep + qsize > first:
+                return True
+    return False
 
 
 def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, grad_scale=1.0, steps=5,
@@ -456,6 +477,6 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
 
     params, grads: matrices [M, N] (rows may be strided, elements of a row adjacent), or convolution weights [Co, Ci, kh, kw], contiguous or
     channels-last, taken as [Co, Ci kh kw]; float32, bfloat16 or float16, one type a call.  momenta: float32 of the same shape and order,
-    contiguous.  What is written may not overlap.  The stored momentum and the whole update are fp32; weights are rounded once.
-    steps, coefficients, eps, joined: as for `orthogonalise`."""
+    contiguous.  What is written may overlap nothing else of the call (rows of one tensor may lie between another's).  The stored momentum
+    and the whole update are fp32; weights are rounded once.  steps, coefficients, eps, joined: as for `orthogonalise`."""
     MuonUpdate(params, grads, momenta, momentum, nesterov, weight_decay, scale, grad_scale, steps, coefficients, eps, joined).step(lr)
