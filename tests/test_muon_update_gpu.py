@@ -30,3 +30,17 @@ def test_a_graph_that_saved_a_weight_before_the_step_is_refused(dev):
         old = t[0].clone()
         ops.muon_step([t[0]], [t[1]], [t[2]], 0.1)
         assert not torch.equal(t[0], old)
+
+
+@pytest.mark.parametrize('order', [1, -1])
+def test_a_large_matrix_beside_a_long_batch_of_small_ones(dev, order):
+    """Together they would pass the largest grid of the norm's launch."""
+    big, small = torch.randn(2048, 2048, device=dev), torch.randn(70000, 1, 1, device=dev)
+    got = ops.orthogonalise([big, small][::order])[::order]
+    assert torch.equal(got[0], ops.orthogonalise(big))
+    a, b, c = ops.NS_COEFFICIENTS           # (the smallest of 70000 normal samples is some 1e-5: eps counts a little)
+    y = small.double() / (small.double().abs() + 1e-7)
+    for _ in range(5):
+        y = y * (a + b * y ** 2 + c * y ** 4)
+    # a step multiplies a relative error by at most |1 + 2 (b A + 2 c A^2) / (a + b A + c A^2)| < 8 for y of 0.5 .. 1.2; pairs of 22 bits
+    assert float((got[1].double() - y).abs().max()) < 2e-4

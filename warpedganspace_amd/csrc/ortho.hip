@@ -1365,8 +1365,15 @@ Plan plan_of(int dtype, bool step, int steps, const wgs_matrix* mats, int count)
 }
 
 constexpr int64_t CHUNK_BYTES = 4LL << 30;       // planes of the matrices that go through the launches together
+// Workgroups of 512 of the norm's launch: a grid has fewer than 2^32 threads.  (All matrices of a run take the largest one's number of parts: without
+// the limit one of 2048^2 beside a batch of 33000 single entries would pass it.)
+constexpr int64_t NORM_BLOCKS = 1 << 22;
+int norm_blocks(int64_t elements) {               // 64 elements a thread where the matrix is large
+    const int64_t sb = elements / 16384;
+    return sb < 1 ? 1 : (sb > STAT_BLOCKS ? STAT_BLOCKS : (int)sb);
+}
 
-// The matrices in runs of at most MAX_MATS entries and CHUNK_BYTES (or one matrix); batches are cut where they have to be.
+// The matrices in runs of at most MAX_MATS entries, NORM_BLOCKS and CHUNK_BYTES (or one matrix); batches are cut where they have to be.
 struct Cursor { int entry = 0, done = 0; };
 int64_t next_chunk(const wgs_matrix* mats, int count, const Plan& p, Cursor& c, Group& g) {
     int64_t bytes = 0;
@@ -1379,8 +1386,12 @@ int64_t next_chunk(const wgs_matrix* mats, int count, const Plan& p, Cursor& c, 
         const Dims d = dims_of(w.rows, w.cols);
         int64_t one = instance_bytes(d, p.npx, p.nt, p.ns);
         if (is_small(d) && small_bytes(d) > one) one = small_bytes(d);
+        const int64_t elements = (int64_t)w.rows * w.cols, largest = elements > most ? elements : most;
         int64_t fit = (CHUNK_BYTES - bytes) / one;
-        if (fit < 1) { if (g.count) break; fit = 1; }
+        if (fit < 1 && !g.count) fit = 1;
+        const int64_t room = NORM_BLOCKS / norm_blocks(largest) - g.instances;
+        if (fit > room) fit = room;
+        if (fit < 1) break;
         const int take = fit < left ? (int)fit : left;
         Mat& m = g.mat[g.count++];
         m.in_bs = w.in_batch_stride; m.out_bs = w.out_batch_stride;
@@ -1394,14 +1405,13 @@ int64_t next_chunk(const wgs_matrix* mats, int count, const Plan& p, Cursor& c, 
         if (w.momentum) m.momentum = w.momentum + (int64_t)c.done * w.rows * w.cols;
         g.instances += take;
         bytes += one * take;
-        if ((int64_t)w.rows * w.cols > most) most = (int64_t)w.rows * w.cols;
+        most = largest;
         c.done += take;
         if (c.done == w.batch) { ++c.entry; c.done = 0; }
         if (take < left) break;
     }
     if (!g.count) return 0;
-    int64_t sb = most / 16384;                    // 64 elements a thread where the matrix is large
-    g.stat_blocks = sb < 1 ? 1 : (sb > STAT_BLOCKS ? STAT_BLOCKS : (int)sb);
+    g.stat_blocks = norm_blocks(most);
     g.info = up((int64_t)g.instances * g.stat_blocks * (int64_t)sizeof(Part), 256);
     int64_t head = g.info + up((int64_t)g.instances * INFO * 4, 256);
     g.part = 0;
