@@ -4,7 +4,7 @@ import struct
 
 import pytest
 
-from tests.test_operator_refusals_cpu import matrix, ortho, refused
+from tests.test_operator_refusals_cpu import I64, P, matrix, ortho, refused
 from warpedganspace_amd import _lib as L
 from warpedganspace_amd import ops
 
@@ -87,3 +87,11 @@ def test_a_large_matrix_beside_a_long_batch_of_small_ones_is_cut_into_runs(order
     assert need(small) < 70000 * (one + 64)                          # one partial norm each: a single run
     # in the large one's run at most 2^14 instances; the rest goes without it
     assert need(big, small) <= max(need(big) + (1 << 14) * (one + 64) + (16 << 22), need(small))
+
+
+def test_label_logprobs_backward_refuses_more_workgroups_than_a_grid_holds():
+    """256 threads a workgroup, fewer than 2^32 threads a grid: 2^23 rows of two parts (over 1024 16-byte vectors) are too many."""
+    def bwd(rows, V):
+        return L.lib().wgs_label_logprobs_bwd(P, 1, I64(rows), I64(V), I64(V), P, I64(-100), P, P, 0, None, P, None, None, P, I64(V), None)
+    refused(bwd(1 << 23, 8200), b'too many scores')
+    refused(bwd((1 << 24) - 1, 16384), b'too many scores')

@@ -533,7 +533,7 @@ int wgs_label_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t 
     const int nv = wgs_cdiv(V, dtype == WGS_F32 ? 4 : 8);
     a.per = UNROLL * 256;
     a.parts = wgs_cdiv(nv, a.per);
-    WGS_CHECK_ARG(rows * a.parts < (1LL << 31), "wgs_label_logprobs_bwd: too many scores for one launch");
+    WGS_CHECK_ARG(rows * a.parts < (1LL << 24), "wgs_label_logprobs_bwd: too many scores for one launch");      // (a grid has fewer than 2^32 threads)
     hipStream_t st = (hipStream_t)stream;
     const dim3 gr((unsigned)(rows * a.parts));
     if (dtype == WGS_F32) WGS_LAUNCH(logprob_bwd_kernel<WGS_F32>, gr, dim3(256), 0, st, a);
