@@ -44,3 +44,28 @@ def test_a_large_matrix_beside_a_long_batch_of_small_ones(dev, order):
         y = y * (a + b * y ** 2 + c * y ** 4)
     # a step multiplies a relative error by at most |1 + 2 (b A + 2 c A^2) / (a + b A + c A^2)| < 8 for y of 0.5 .. 1.2; pairs of 22 bits
     assert float((got[1].double() - y).abs().max()) < 2e-4
+
+
+def test_a_gradient_that_was_made_anew_is_not_taken_for_the_old_one(dev):
+    w = torch.randn(6, 9, device=dev, requires_grad=True)
+    x = torch.randn(9, 4, device=dev)
+    m = torch.zeros(6, 9, device=dev)
+    (w @ x).sum().backward()
+    plan = ops.MuonUpdate([w], [w.grad], [m])
+    plan.step(0.1)
+    w.grad.zero_()                             # zero_grad(set_to_none=False): the same tensor
+    (w @ x).sum().backward()
+    plan.step(0.1)
+    old = w.detach().clone()
+    for again in (False, True):
+        w.grad = None                          # zero_grad(): the next backward makes a new tensor
+        if again:
+            (w @ x).sum().backward()
+        with pytest.raises(L.WgsError, match='another tensor'):
+            plan.step(0.1)
+    assert torch.equal(w, old)
+    ops.MuonUpdate([w], [w.grad], [m]).step(0.1)
+    g = torch.randn(6, 9, device=dev)          # a gradient of one's own: .grad does not matter
+    plan = ops.MuonUpdate([w], [g], [m])
+    w.grad = None
+    plan.step(0.1)

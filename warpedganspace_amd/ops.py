@@ -354,7 +354,8 @@ class MuonUpdate:
     """The step of `muon_step` on tensors that stay where they are: checked and described once, then `step(lr)` any number of times.
 
     It keeps the tensors themselves (and so their memory), not results: every call reads the gradients and updates momenta and weights in place,
-    on the current stream of their device; its workspace comes from torch's allocator, call by call."""
+    on the current stream of their device; its workspace comes from torch's allocator, call by call.  A step is refused once a tensor has other memory,
+    or once a gradient that was its param's .grad is so no longer (zero_grad(set_to_none=True) and the next backward make a new one)."""
 
     def __init__(self, params, grads, momenta, momentum=0.95, nesterov=True, weight_decay=0.0, scale=None, grad_scale=1.0, steps=5,
                  coefficients=NS_COEFFICIENTS, eps=1e-7, joined=None):
@@ -406,6 +407,7 @@ class MuonUpdate:
         self.code = _DTYPES[dtype]
         self.need = L.lib().wgs_muon_step_ws_bytes(self.mats, self.n, self.code, self.steps)
         self.places = self._places()
+        self.own = [(w, g) for w, g in zip(params, grads) if w.is_leaf and w.grad is g]
         self.lr = None
 
     def _places(self):
@@ -417,6 +419,9 @@ class MuonUpdate:
             return
         if self._places() != self.places:
             raise L.WgsError("MuonUpdate: a tensor has been given other memory since it was described: make a new one")
+        if any(w.grad is not g for w, g in self.own):
+            raise L.WgsError("MuonUpdate: a param's .grad is another tensor than the one described: make a new one, or keep the gradients "
+                             "(zero_grad(set_to_none=False))")
         lr = float(lr)                          # (a tensor may change in place)
         if lr != self.lr:
             decay = 1.0 - lr * self.weight_decay
