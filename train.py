@@ -16,6 +16,7 @@ import torch.distributed as dist
 from warpedganspace_amd.aux import create_exp_dir, exp_dir_name
 from warpedganspace_amd.config import GAN_RESOLUTIONS, GAN_WEIGHTS, RECONSTRUCTOR_TYPES
 from warpedganspace_amd.gan_load import build_gan
+from warpedganspace_amd.ops import TOP_MAX
 from warpedganspace_amd.reconstructor import Reconstructor
 from warpedganspace_amd.support_sets import SupportSets
 from warpedganspace_amd.trainer import Trainer
@@ -65,8 +66,11 @@ def parse(argv=None):
                      help="update of the reconstructor's convolution weights: adam = the reference's; muon = orthogonalised momentum, steps of "
                           "the size of Adam's at --reconstructor-lr (all other parameters: Adam)")
     ext.add_argument('--lambda-ent', type=float, default=0.0, help="weight of the mean entropy of the path scores, subtracted from the loss")
-    ext.add_argument('--label-top', type=int, default=0, metavar='K', help="report the accuracy of the K most likely paths too (0 = off)")
-    return p.parse_args(argv)
+    ext.add_argument('--label-top', type=int, default=0, metavar='K', help="report the accuracy of the K most likely paths too (0 = off; at most 64 and -K)")
+    args = p.parse_args(argv)
+    if not 0 <= args.label_top <= min(TOP_MAX, args.num_support_sets or TOP_MAX):
+        p.error("argument --label-top: must be 0 .. {} and at most the number of support sets, got {}".format(TOP_MAX, args.label_top))
+    return args
 
 
 def main(argv=None):

@@ -203,7 +203,10 @@ class TrainStep:
         if self.optimizer not in ('adam', 'muon'):
             raise ValueError("optimizer must be 'adam' or 'muon', got %r" % (self.optimizer,))
         self.lambda_ent = float(getattr(params, 'lambda_ent', 0.0) or 0.0)      # total loss -= lambda_ent * mean entropy of the path scores
-        self.label_top = min(int(getattr(params, 'label_top', 0) or 0), support_sets.ALPHAS.shape[0], ops.TOP_MAX)      # top-k accuracy statistic
+        self.label_top = int(getattr(params, 'label_top', 0) or 0)              # top-k accuracy statistic
+        if not 0 <= self.label_top <= min(support_sets.ALPHAS.shape[0], ops.TOP_MAX):
+            raise ValueError("label_top must be 0 .. %d (and at most the number of support sets, %d), got %d" % (
+                ops.TOP_MAX, support_sets.ALPHAS.shape[0], self.label_top))
         self.extra_sum = torch.zeros(2, device=device)                          # (mean entropy, top-k accuracy) since the last pop_stats
         self.bucket = FlatBucket([(params.reconstructor_lr, r_params), (params.support_set_lr, s_params)], device, muon=self.optimizer == 'muon')
         if world > 1:
