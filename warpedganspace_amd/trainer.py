@@ -660,22 +660,19 @@ class TrainStep:
             self.extra_sum[1] += (r.top_index == idx[:, None]).any(1).float().mean()
 
     def pop_stats(self):
-        """Mean (accuracy, classification_loss, regression_loss, total_loss) since the last call (one sync)."""
-        s = self.stats_sum.clone()
+        """Mean (accuracy, classification_loss, regression_loss, total_loss) since the last call, and the optional terms' entropy and top-k accuracy
+        (one sync, and one all-reduce when world > 1)."""
+        extra = bool(self.lambda_ent or self.label_top)
+        s = torch.cat([self.stats_sum, self.extra_sum]) if extra else self.stats_sum.clone()
         if self.world > 1:
             dist.all_reduce(s)
             s /= self.world
         v = (s / max(self.stats_n, 1)).tolist()
         out = {'accuracy': v[3], 'classification_loss': v[0], 'regression_loss': v[1], 'total_loss': v[2]}
-        if self.lambda_ent or self.label_top:
-            e = self.extra_sum.clone()
-            if self.world > 1:
-                dist.all_reduce(e)
-                e /= self.world
-            e = (e / max(self.stats_n, 1)).tolist()
-            out['entropy'] = e[0]
+        if extra:
+            out['entropy'] = v[4]
             if self.label_top:
-                out['top%d_accuracy' % self.label_top] = e[1]
+                out['top%d_accuracy' % self.label_top] = v[5]
             self.extra_sum.zero_()
         self.stats_sum.zero_()
         self.stats_n = 0
