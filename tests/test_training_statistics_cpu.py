@@ -10,3 +10,21 @@ def test_command_line_refuses_more_alternatives_than_there_are(args, capsys):
     assert '--label-top' in capsys.readouterr().err
     assert train.parse(['--gan-type', 'StyleGAN2', '-K', '8', '--label-top', '8']).label_top == 8
     assert train.parse(['--gan-type', 'StyleGAN2', '--label-top', '64']).label_top == 64
+
+
+def test_the_log_shows_the_optional_statistics(tmp_path, capsys, monkeypatch):
+    import types
+    from warpedganspace_amd import trainer as T
+    p = types.SimpleNamespace(tensorboard=False, batch_size=4, max_iter=10)
+    tr = T.Trainer(params=p, exp_dir='exp', root=str(tmp_path))
+    stats = {'accuracy': 0.5, 'classification_loss': 1.0, 'regression_loss': 0.25, 'total_loss': 1.25}
+    moved = []
+    monkeypatch.setattr(T, 'update_stdout', moved.append)
+    tr.log_progress(1, 0.1, 1.0, 9.0, stats)
+    plain = capsys.readouterr().out
+    monkeypatch.setattr(T.sys.stdout, 'isatty', lambda: True, raising=False)
+    tr.log_progress(2, 0.1, 1.0, 9.0, dict(stats, entropy=2.125, top5_accuracy=0.75))
+    more = capsys.readouterr().out
+    assert 'ntropy' not in plain and '2.125' in more and 'Entropy' in more and 'Top5 accuracy' in more and '0.75' in more
+    assert len(more.splitlines()) == len(plain.splitlines()) + 2
+    assert moved[-1:] == [12]                   # the block that the next log overwrites

@@ -753,13 +753,16 @@ class Trainer(object):
         print("      \\__Classification loss : {:.08f}".format(stats['classification_loss']))
         print("      \\__Regression loss     : {:.08f}".format(stats['regression_loss']))
         print("      \\__Total loss          : {:.08f}".format(stats['total_loss']))
+        more = [key for key in stats if key not in ('accuracy', 'classification_loss', 'regression_loss', 'total_loss')]
+        for key in more:                        # the optional terms' statistics
+            print("      \\__{:<20}: {:.08f}".format(key.replace('_', ' ').capitalize(), stats[key]))
         print("         ===================================================================")
         print("      \\__Mean iter time      : {:.3f} sec".format(mean_iter_time))
         print("      \\__Elapsed time        : {}".format(sec2dhms(elapsed_time)))
         print("      \\__ETA                 : {}".format(sec2dhms(eta)))
         print("         ===================================================================")
         if sys.stdout.isatty():
-            update_stdout(10)
+            update_stdout(10 + len(more))
 
     def agree_tensorboard(self, device=None):
         """Rank 0's "a TensorBoard writer exists" broadcast to every rank (the writer is rank 0's alone, and creating it can fail there:
