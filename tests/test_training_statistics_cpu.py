@@ -28,3 +28,19 @@ def test_the_log_shows_the_optional_statistics(tmp_path, capsys, monkeypatch):
     assert 'ntropy' not in plain and '2.125' in more and 'Entropy' in more and 'Top5 accuracy' in more and '0.75' in more
     assert len(more.splitlines()) == len(plain.splitlines()) + 2
     assert moved[-1:] == [12]                   # the block that the next log overwrites
+
+
+def test_moments_of_another_optimizer_are_not_dropped_without_a_word(tmp_path, capsys):
+    import types
+    from warpedganspace_amd.trainer import Trainer
+    tr = Trainer(params=types.SimpleNamespace(tensorboard=False), exp_dir='exp', root=str(tmp_path))
+    engine = types.SimpleNamespace(optimizer='muon', bucket=types.SimpleNamespace(step_count=7), load_optim_state=lambda st: st.get('optimizer') == 'muon')
+    tr.restore_optim(engine)
+    assert capsys.readouterr().out == ''
+    tr.resume_optim = {'optimizer': 'muon'}
+    tr.restore_optim(engine)
+    assert 'Restored momentum and Adam moments (step 7)' in capsys.readouterr().out
+    tr.resume_optim = {'step': 3}               # written before the key existed: Adam's
+    tr.restore_optim(engine)
+    out = capsys.readouterr().out
+    assert 'optimizer adam' in out and 'optimizer muon' in out and 'fresh' in out

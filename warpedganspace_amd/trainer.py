@@ -777,6 +777,21 @@ class Trainer(object):
         self.tb_active = bool(flag)
         return self.tb_active
 
+    def restore_optim(self, engine):
+        """The checkpoint's moments into the engine; one written with another --optimizer (or for other parameters) starts from fresh ones, and
+        says so."""
+        state = getattr(self, 'resume_optim', None)
+        if state is None:
+            return
+        restored = engine.load_optim_state(state)
+        if self.rank == 0:
+            if restored:
+                print("#. Restored {} moments (step {}) from the checkpoint".format('Adam' if engine.optimizer == 'adam' else 'momentum and Adam',
+                                                                                    engine.bucket.step_count))
+            else:
+                print("#. The checkpoint's moments (optimizer {}) do not fit this run's (optimizer {}): starting from fresh ones".format(
+                    state.get('optimizer', 'adam'), engine.optimizer))
+
     def stats_due(self, iteration):
         """True in the iterations whose statistics are popped (one device sync + one all-reduce when world > 1): a function of
         rank-invariant state only."""
@@ -834,8 +849,7 @@ class Trainer(object):
             print("#. Generator arithmetic calibrated on this generator ({} latent codes against the exact-fp32 kernels): per-layer table '{}' "
                   "({} fp16-rounded layer(s)); rungs tried (worst single image, codes seen): {}".format(
                       c['images'], c['table'], c['fp16_layers'], ', '.join("%s %.2e (%d)" % tuple(t) for t in c['tried'])))
-        if getattr(self, 'resume_optim', None) is not None and engine.load_optim_state(self.resume_optim) and self.rank == 0:
-            print("#. Restored Adam moments (step {}) from the checkpoint".format(engine.bucket.step_count))
+        self.restore_optim(engine)
         if self.rank == 0:
             print("#. Start training from iteration {}".format(starting_iter))
         self.agree_tensorboard(dev)
