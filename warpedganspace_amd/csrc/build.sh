@@ -3,10 +3,9 @@
 set -euo pipefail
 cd "$(dirname "$0")"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wall -Wno-unused-function"
-# No packed fp32 instructions from the compiler: some of their forms have given wrong results now and then.  (hipcc's host pass warns that it
-# does not know the feature.)  conv_wino_f32.hip writes its own packed transforms.
-NOPK="-Xclang -target-feature -Xclang -packed-fp32-ops"
+# No packed fp32 instructions (v_pk_add_f32 and the like), from the compiler or by hand: some of their forms have given wrong results now and then on
+# gfx950, without an error.  (hipcc's host pass warns that it does not know the feature.)
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops"
 OBJS=()
 for src in *.hip; do
   obj="build/${src%.hip}.o"
@@ -14,8 +13,7 @@ for src in *.hip; do
   if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ wgs_common.h -nt "$obj" ] || [ conv_args.h -nt "$obj" ] || [ fir4.h -nt "$obj" ] || [ conv_epilogue.h -nt "$obj" ] || [ conv_scheme.h -nt "$obj" ] || [ conv_nt_kernel.inc -nt "$obj" ] || [ conv_nt_launch.inc -nt "$obj" ] || [ ../../include/wgs.h -nt "$obj" ] \
      || { [ -f "${src%.hip}.inc" ] && [ "${src%.hip}.inc" -nt "$obj" ]; }; then
     echo "[hipcc] $src"
-    if grep -q 'asm.*"v_pk_[a-z]*_f32' "$src"; then $HIPCC $FLAGS -c "$src" -o "$obj" &
-    else $HIPCC $FLAGS $NOPK -c "$src" -o "$obj" & fi
+    $HIPCC $FLAGS -c "$src" -o "$obj" &
   fi
   OBJS+=("$obj")
 done

@@ -365,7 +365,7 @@ __global__ __launch_bounds__(32 * GH, GH == 8 ? 2 : 1) void upconv_blur_kernel(c
             dev = fmaxf(dev, fabsf(kf[i] - kv[i >> 2] * kh[i & 3]));
         }
         sep = sep && dev <= 2e-7f * kmax;
-        // uniform values: as scalar registers the eight taps feed the packed FMAs through op_sel (no {k, k} vector pairs: 16 registers fewer in
+        // uniform values: the eight taps as scalar registers, which the FMAs read directly (no vector copies: registers saved in
         // the blur, which runs while the other channel half's 64 accumulators are still live)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(32 * GH, GH == 8 ? 2 : 1) void upconv_blur_kernel(c
                 for (int ph = 0; ph < 4; ++ph) {
                     const int po = ((ph >> 1) * TW + (ph & 1)) * 128;        // the phase's position offset: an immediate of the store
                     unsigned char* tb = reinterpret_cast<unsigned char*>(T) + po;
-                    // (acc * alpha) * column scale for two rows per packed multiply
+                    // (acc * alpha) * column scale, two rows at a time
                     const f32x2 ta = f32x2{half ? acc[ph][1][rg] : acc[ph][0][rg], half ? acc[ph][1][rg + 1] : acc[ph][0][rg + 1]} * al * cs;
                     const f32x2 tc = f32x2{half ? acc[ph][1][rg + 2] : acc[ph][0][rg + 2], half ? acc[ph][1][rg + 3] : acc[ph][0][rg + 3]} * al * cs;
                     *reinterpret_cast<float*>(tb + o0) = ta.x;
@@ -434,8 +434,7 @@ __global__ __launch_bounds__(32 * GH, GH == 8 ? 2 : 1) void upconv_blur_kernel(c
             const float4 sn = *reinterpret_cast<const float4*>(aux_sn + half * 32 + q * 4);
             const int ox = 2 * x0 + lx;
             // finish one output pixel: noise, bias, activation, magnitude, store
-            // (two channels per instruction throughout: v_pk_add / v_pk_mul; the leaky ReLU as max(a, 0.2 a), which equals the
-            //  select for every finite a, signed zeros included)
+            // (the leaky ReLU as max(a, 0.2 a), which equals the select for every finite a, signed zeros included)
             const f32x2 bv0 = {bv.x, bv.y}, bv1 = {bv.z, bv.w}, sn0 = {sn.x, sn.y}, sn1 = {sn.z, sn.w};
             // per-thread row base of the output address, the noise slot and the row bound: a row of the strip then costs one add, one
             // compare and one select (round 6: each emit used to rebuild its address with a 64-bit multiply-add and a 32-bit multiply
@@ -472,8 +471,8 @@ __global__ __launch_bounds__(32 * GH, GH == 8 ? 2 : 1) void upconv_blur_kernel(c
             };
             if (sep) {
                 // separable kernel (StyleGAN2's [1,3,3,1] outer product): horizontal pass on each loaded row, vertical pass over a
-                // four-row window of the results: 8 instead of 16 multiply-adds per output and channel — as PACKED fp32 FMAs
-                // (v_pk_fma_f32: two channels per instruction; the epilogue is a third of this kernel and pure vector work)
+                // four-row window of the results: 8 instead of 16 multiply-adds per output and channel
+                // (the epilogue is a third of this kernel and pure vector work)
                 f32x2 hlo[4], hhi[4];
 #pragma unroll
                 for (int rr = 0; rr < RS + 3; ++rr) {

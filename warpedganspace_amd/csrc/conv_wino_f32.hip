@@ -79,11 +79,21 @@ __device__ __forceinline__ f32x4 buf_load4(const __amdgpu_buffer_rsrc_t r, int v
     const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0);
     return __builtin_bit_cast(f32x4, v);
 }
-// The transform's arithmetic written as the instructions it is (the backend splits 4-vectors into scalars and keeps a quad permute
-// as a separate v_mov_b32_dpp): packed fp32 adds / multiplies on register pairs ...
-__device__ __forceinline__ f32x2 pk_add(f32x2 a, f32x2 b) { f32x2 d; asm("v_pk_add_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b)); return d; }
-__device__ __forceinline__ f32x2 pk_sub(f32x2 a, f32x2 b) { f32x2 d; asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(d) : "v"(a), "v"(b)); return d; }
-__device__ __forceinline__ f32x2 pk_mul(f32x2 a, f32x2 b) { f32x2 d; asm("v_pk_mul_f32 %0, %1, %2" : "=v"(d) : "v"(a), "v"(b)); return d; }
+// The transform's arithmetic: adds / multiplies of two channels, each rounded for itself (no fused multiply-adds: the results do not depend on what
+// the compiler would join), in single fp32 instructions (packed ones are not used, see build.sh; they gave
+// the same bits, and the fp32w step 601.0 img/s against 600.4) ...
+__device__ __forceinline__ f32x2 pair_add(f32x2 a, f32x2 b) {
+#pragma clang fp contract(off)
+    return a + b;
+}
+__device__ __forceinline__ f32x2 pair_sub(f32x2 a, f32x2 b) {
+#pragma clang fp contract(off)
+    return a - b;
+}
+__device__ __forceinline__ f32x2 pair_mul(f32x2 a, f32x2 b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
 // ... and v += s * (v of lane {2, 2, 1, 1}[lane & 3] of the quad), in place on the four values of a loaded float4 (s_nop 1: a VGPR
 // written by the preceding VALU instruction may not be read through DPP for two cycles)
 __device__ __forceinline__ void quad_row_pass(f32x4& v, float s) {
@@ -214,8 +224,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void wino_f32_kernel(cons
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const f32x2 a = {ra[u][ia][2 * k], ra[u][ia][2 * k + 1]}, bb = {ra[u][ib][2 * k], ra[u][ib][2 * k + 1]};
-            h[k] = xi == 1 ? pk_add(a, bb) : pk_sub(a, bb);
-            if (STY) h[k] = pk_mul(h[k], (f32x2){rsv[u][2 * k], rsv[u][2 * k + 1]});
+            h[k] = xi == 1 ? pair_add(a, bb) : pair_sub(a, bb);
+            if (STY) h[k] = pair_mul(h[k], (f32x2){rsv[u][2 * k], rsv[u][2 * k + 1]});
         }
         const f32x4 v = {h[0][0], h[0][1], h[1][0], h[1][1]};
         *reinterpret_cast<f32x4*>(v_dst[u] + buf * STAGE + xi * 4 * PS) = v;
