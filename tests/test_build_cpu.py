@@ -2,6 +2,9 @@
 import glob
 import os
 import re
+import shutil
+import subprocess
+import time
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'warpedganspace_amd', 'csrc')
 SCRIPT = open(os.path.join(CSRC, 'build.sh')).read()
@@ -16,3 +19,40 @@ def test_no_packed_fp32_instructions():
     assert '-Xclang -target-feature -Xclang -packed-fp32-ops' in flags
     compiles = [ln for ln in SCRIPT.splitlines() if re.search(r'\$HIPCC.* -c ', ln)]
     assert compiles and all('$FLAGS' in ln for ln in compiles)
+
+
+def _copy(tmp_path):
+    """The sources beside a compiler that only leaves an empty output."""
+    csrc = tmp_path / 'pkg' / 'csrc'
+    csrc.mkdir(parents=True)
+    (tmp_path / 'include').mkdir()
+    for f in glob.glob(os.path.join(CSRC, '*')):
+        if os.path.isfile(f):
+            shutil.copy2(f, csrc)
+    shutil.copy2(os.path.join(CSRC, '..', '..', 'include', 'wgs.h'), tmp_path / 'include')
+    cc = tmp_path / 'cc'
+    cc.write_text('#!/bin/sh\nwhile [ $# -gt 0 ]; do if [ "$1" = -o ]; then : > "$2"; fi; shift; done\n')
+    cc.chmod(0o755)
+    return csrc, dict(os.environ, HIPCC=str(cc))
+
+
+def test_a_change_of_the_flags_rebuilds_every_object(tmp_path, monkeypatch):
+    from warpedganspace_amd import _lib as L
+    csrc, env = _copy(tmp_path)
+    monkeypatch.setattr(L, '_HERE', str(csrc.parent))
+    monkeypatch.setattr(L, 'HEADER_PATH', str(tmp_path / 'include' / 'wgs.h'))
+    monkeypatch.setattr(L, 'LIB_PATH', str(csrc.parent / 'libwgs_hip.so'))
+
+    def build():
+        out = subprocess.run(['bash', str(csrc / 'build.sh')], env=env, check=True, capture_output=True, text=True).stdout
+        assert L.library_matches_sources() is True
+        return out.count('[hipcc]')
+    sources = len(glob.glob(str(csrc / '*.hip')))
+    assert build() == sources
+    assert build() == 0
+    script = csrc / 'build.sh'
+    script.write_text(script.read_text().replace('-O3', '-O2'))
+    assert L.library_matches_sources() is False
+    later = time.time() + 60
+    os.utime(script, (later, later))
+    assert build() == sources

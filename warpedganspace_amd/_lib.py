@@ -28,7 +28,8 @@ def header_symbols(header_path=HEADER_PATH):
 
 
 def source_fingerprint():
-    """sha256 over csrc/*.hip, *.h, *.inc and include/wgs.h in the order build.sh hashes them (shell glob order = sorted names)."""
+    """sha256 over csrc/*.hip, *.h, *.inc, include/wgs.h and csrc/build.sh (its flags) in the order build.sh hashes them (shell glob order =
+    sorted names)."""
     import glob
     import hashlib
     csrc = os.path.join(_HERE, "csrc")
@@ -37,6 +38,7 @@ def source_fingerprint():
         for f in sorted(glob.glob(os.path.join(csrc, pat))):
             h.update(open(f, "rb").read())
     h.update(open(HEADER_PATH, "rb").read())
+    h.update(open(os.path.join(csrc, "build.sh"), "rb").read())
     return h.hexdigest()
 
 

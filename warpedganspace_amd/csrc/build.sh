@@ -10,7 +10,7 @@ OBJS=()
 for src in *.hip; do
   obj="build/${src%.hip}.o"
   mkdir -p build
-  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ wgs_common.h -nt "$obj" ] || [ conv_args.h -nt "$obj" ] || [ fir4.h -nt "$obj" ] || [ conv_epilogue.h -nt "$obj" ] || [ conv_scheme.h -nt "$obj" ] || [ conv_nt_kernel.inc -nt "$obj" ] || [ conv_nt_launch.inc -nt "$obj" ] || [ ../../include/wgs.h -nt "$obj" ] \
+  if [ ! -f "$obj" ] || [ "$src" -nt "$obj" ] || [ wgs_common.h -nt "$obj" ] || [ conv_args.h -nt "$obj" ] || [ fir4.h -nt "$obj" ] || [ conv_epilogue.h -nt "$obj" ] || [ conv_scheme.h -nt "$obj" ] || [ conv_nt_kernel.inc -nt "$obj" ] || [ conv_nt_launch.inc -nt "$obj" ] || [ ../../include/wgs.h -nt "$obj" ] || [ build.sh -nt "$obj" ] \
      || { [ -f "${src%.hip}.inc" ] && [ "${src%.hip}.inc" -nt "$obj" ]; }; then
     echo "[hipcc] $src"
     $HIPCC $FLAGS -c "$src" -o "$obj" &
@@ -19,7 +19,7 @@ for src in *.hip; do
 done
 wait
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o ../libwgs_hip.so "${OBJS[@]}"
-# fingerprint of the sources this library was built from (checked by __graft_entry__.build() and warpedganspace_amd._lib: a prebuilt
+# fingerprint of the sources and flags this library was built from (checked by __graft_entry__.build() and warpedganspace_amd._lib: a prebuilt
 # .so that travels with a snapshot must match the sources beside it)
-LC_ALL=C; export LC_ALL; cat *.hip *.h *.inc ../../include/wgs.h | sha256sum | cut -d' ' -f1 > ../libwgs_hip.so.sources.sha256
+LC_ALL=C; export LC_ALL; cat *.hip *.h *.inc ../../include/wgs.h build.sh | sha256sum | cut -d' ' -f1 > ../libwgs_hip.so.sources.sha256
 echo "built $(cd .. && pwd)/libwgs_hip.so"
