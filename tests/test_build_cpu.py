@@ -56,3 +56,22 @@ def test_a_change_of_the_flags_rebuilds_every_object(tmp_path, monkeypatch):
     later = time.time() + 60
     os.utime(script, (later, later))
     assert build() == sources
+
+
+def test_a_failed_compilation_ends_the_build(tmp_path):
+    """Not linked from an older object: the next run compiles that source again."""
+    csrc, env = _copy(tmp_path)
+    run = ['bash', str(csrc / 'build.sh')]
+    subprocess.run(run, env=env, check=True, capture_output=True)
+    library = csrc.parent / 'libwgs_hip.so'
+    library.unlink()
+    later = time.time() + 60
+    os.utime(csrc / 'core.hip', (later, later))
+    cc = tmp_path / 'cc'
+    good = cc.read_text()
+    cc.write_text(good.replace('#!/bin/sh\n', '#!/bin/sh\ncase "$*" in *core.hip*) exit 1;; esac\n'))
+    assert subprocess.run(run, env=env, capture_output=True).returncode != 0
+    assert not library.exists() and not (csrc / 'build' / 'core.o').exists()
+    cc.write_text(good)
+    out = subprocess.run(run, env=env, check=True, capture_output=True, text=True).stdout
+    assert out.count('[hipcc]') == 1 and library.exists()
