@@ -136,8 +136,9 @@ def timed_steps(eng, steps, warmup, world, dev):
     barrier()
     dt = time.perf_counter() - t0
     if world > 1:
+        from warpedganspace_amd.trainer import all_reduce
         t = torch.tensor([dt], device=dev, dtype=torch.float64)
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        all_reduce(t, op=dist.ReduceOp.MAX)
         dt = float(t.item())
     return dt
 

@@ -44,3 +44,54 @@ def test_moments_of_another_optimizer_are_not_dropped_without_a_word(tmp_path, c
     tr.restore_optim(engine)
     out = capsys.readouterr().out
     assert 'optimizer adam' in out and 'optimizer muon' in out and 'fresh' in out
+
+
+def test_gloo_is_given_host_tensors_only(monkeypatch):
+    """A stand-in for a device tensor: the collective gets its copy in host memory, and the result is copied back."""
+    import torch
+    from warpedganspace_amd import trainer as T
+    calls = []
+
+    class OnDevice:
+        is_cuda = True
+
+        def __init__(self, v):
+            self.v = v
+
+        def detach(self):
+            return self
+
+        def cpu(self):
+            return self.v.clone()
+
+        def copy_(self, h):
+            self.v = h.clone()
+
+    def reduce(t, op=None, async_op=False):
+        calls.append((type(t), async_op))
+        if isinstance(t, torch.Tensor):
+            t *= 3
+        return 'work' if async_op else None
+
+    def spread(t, src):
+        calls.append((type(t), src))
+        if isinstance(t, torch.Tensor):
+            t.fill_(7)
+    backend = ['gloo']
+    monkeypatch.setattr(T.dist, 'get_backend', lambda: backend[0])
+    monkeypatch.setattr(T.dist, 'all_reduce', reduce)
+    monkeypatch.setattr(T.dist, 'broadcast', spread)
+    d = OnDevice(torch.tensor([1.0, 2.0]))
+    T.all_reduce(d)
+    assert d.v.tolist() == [3.0, 6.0]
+    T.all_reduce(d, async_op=True).wait()
+    assert d.v.tolist() == [9.0, 18.0]
+    T.broadcast(d, 0)
+    assert d.v.tolist() == [7.0, 7.0] and calls == [(torch.Tensor, False), (torch.Tensor, False), (torch.Tensor, 0)]
+    del calls[:]
+    h = torch.ones(2)
+    assert T.all_reduce(h, async_op=True) == 'work'                  # host tensors and RCCL: as they are
+    backend[0] = 'nccl'
+    T.all_reduce(d)
+    T.broadcast(d, 1)
+    assert calls == [(torch.Tensor, True), (OnDevice, False), (OnDevice, 1)]

@@ -34,6 +34,38 @@ from .aux import TrainingStatTracker, sample_z, sec2dhms, update_progress, updat
 from .support_sets import rbf_workspace
 
 
+class _Finished:
+    """Handle of a collective that is complete."""
+
+    def wait(self):
+        return True
+
+
+def _on_host(t):
+    """Whether a collective of t goes through host memory: every backend but RCCL is given host tensors only.  (gloo's collectives on device tensors
+    run copies on streams of their own; with several ranks on one GPU they have hung, and lost processes.)"""
+    return t.is_cuda and dist.get_backend() != 'nccl'
+
+
+def all_reduce(t, async_op=False, op=dist.ReduceOp.SUM):
+    """dist.all_reduce of a tensor wherever it is; through host memory: a copy out that is waited for, the collective, and a copy back."""
+    if not _on_host(t):
+        return dist.all_reduce(t, op=op, async_op=async_op)
+    h = t.detach().cpu()
+    dist.all_reduce(h, op=op)
+    t.copy_(h)
+    return _Finished() if async_op else None
+
+
+def broadcast(t, src):
+    """dist.broadcast of a tensor wherever it is (see all_reduce)."""
+    if not _on_host(t):
+        return dist.broadcast(t, src)
+    h = t.detach().cpu()
+    dist.broadcast(h, src)
+    t.copy_(h)
+
+
 def sampler_seed(seed, rank, world, start_iter, device):
     """Seed of this rank's device-side sampler.  Every rank must draw DIFFERENT (z, idx, magnitude) samples (the global
     batch is the union of the ranks' local batches), an unseeded run must not repeat the previous run's sequence (the
@@ -211,10 +243,10 @@ class TrainStep:
         self.bucket = FlatBucket([(params.reconstructor_lr, r_params), (params.support_set_lr, s_params)], device, muon=self.optimizer == 'muon')
         if world > 1:
             # replicas start from rank 0's parameters and BN running statistics, whatever each rank's RNG produced
-            dist.broadcast(self.bucket.flat, 0)
+            broadcast(self.bucket.flat, 0)
             for b in reconstructor.buffers():
                 if b.is_floating_point():
-                    dist.broadcast(b.data, 0)
+                    broadcast(b.data, 0)
         K, n2 = support_sets.ALPHAS.shape
         self.K, self.n2, self.d = K, n2, support_sets.support_vectors_dim
         # the RBF kernels stream 16-byte vectors: a latent dimension that is not a multiple of 4 (BigGAN-256 / -512 truncate
@@ -593,7 +625,7 @@ class TrainStep:
                     # R's gradients (the first bucket group, 47 MB at cfg3) are final after these launches: their all-reduce
                     # is queued behind them and overlaps the generator's backward (no trainable parameters)
                     _, a, b = self.bucket.groups[0]
-                    pending.append(dist.all_reduce(self.bucket.grad[a:b], async_op=True))
+                    pending.append(all_reduce(self.bucket.grad[a:b], async_op=True))
         if deferred is not None:
             if self.wgrad_hook_res and hookable and self.world == 1:
                 hooks.append((self.wgrad_hook_res, run_wgrads))     # under the backward's latency-bound tail instead of next to its chip-filling layers
@@ -602,7 +634,7 @@ class TrainStep:
             del deferred
         elif self.world > 1:
             _, a, b = self.bucket.groups[0]
-            pending.append(dist.all_reduce(self.bucket.grad[a:b], async_op=True))
+            pending.append(all_reduce(self.bucket.grad[a:b], async_op=True))
         if tail is not None:
             hooks.append((self.tail_hook_res, tail))      # (a generator without hooks: run after its backward, below)
         try:
@@ -629,7 +661,7 @@ class TrainStep:
             cur.wait_stream(side)                                             # deferred weight gradients (and their all-reduce)
         if self.world > 1:
             _, a, b = self.bucket.groups[1]                                   # S's gradients (RCCL sum; Adam divides by world)
-            pending.append(dist.all_reduce(self.bucket.grad[a:b], async_op=True))
+            pending.append(all_reduce(self.bucket.grad[a:b], async_op=True))
             ev = self.comm_events
             if ev is not None:      # bench.py: how long the main stream sits in front of the collectives (exposed wait)
                 e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -665,7 +697,7 @@ class TrainStep:
         extra = bool(self.lambda_ent or self.label_top)
         s = torch.cat([self.stats_sum, self.extra_sum]) if extra else self.stats_sum.clone()
         if self.world > 1:
-            dist.all_reduce(s)
+            all_reduce(s)
             s /= self.world
         v = (s / max(self.stats_n, 1)).tolist()
         out = {'accuracy': v[3], 'classification_loss': v[0], 'regression_loss': v[1], 'total_loss': v[2]}
@@ -829,7 +861,7 @@ class Trainer(object):
         starting_iter = self.get_starting_iteration(support_sets, reconstructor)
         if self.world > 1:   # identical replicas on every rank
             for t in list(support_sets.parameters()) + list(reconstructor.parameters()) + list(reconstructor.buffers()):
-                dist.broadcast(t.data, 0)
+                broadcast(t.data, 0)
         if self.ck_iter == p.max_iter:
             print("#. This experiment has already been completed and can be found @ {}".format(self.wip_dir))
             if self.rank == 0:
