@@ -5,8 +5,8 @@
 //   dl_v = g ([v = t] - p_v) - h p_v (log p_v + H) + sum_j q_j ([v = i_j] - p_v)        for upstream (g, h, q) of (logp, H, top_logp)
 //
 // Both directions are HBM-bound: the forward reads the scores once (m, s, u are carried online per lane, rescaled when the lane's maximum
-// rises), the backward reads them once more and writes the gradient.  All statistics are fp32; s and u have at most V / 256 terms a lane before
-// the tree.  Scores are taken relative to m before the exponential, so far-from-zero rows lose nothing.
+// rises), the backward reads them once more and writes the gradient.  All statistics are fp32; s and u have at most V / 256 terms a lane
+// (V / 64 up to 2048 scores) before the tree.  Scores are taken relative to m before the exponential, so far-from-zero rows lose nothing.
 //
 // Alternatives: a score's key = (order-preserving bits << 32 | ~index), so keys are distinct and equal scores sort by the lower index.  Every
 // wave keeps its own sorted list of 64 keys, one a lane, and the key of the `top`-th: a vector of scores costs one comparison of its maximum

@@ -761,8 +761,9 @@ __global__ __launch_bounds__(64 * WAVES_M * WAVES_N, 1) void ortho_gemm_kernel(c
         const Job& j0 = js.job[0];
         asm volatile("" :: "s"(m0.M), "s"(m0.ws), "s"(m0.out), "s"(g.ws), "s"(g.info), "s"(js.sym), "s"(j0.kind), "s"(j0.first), "s"(js.job[1].kind), "s"(total));
     }
-    // Workgroups go round the 8 XCDs: runs of at most 32 tiles in turn, equally many each, so that an XCD's CUs work on neighbouring tiles and the
-    // first entries (the longest sums) are spread over all XCDs.
+    // Workgroups go round the 8 XCDs: runs of at most 32 tiles in turn, equally many each, so that an XCD's CUs work on neighbouring tiles and every
+    // entry is spread over the XCDs.  Entries come in the caller's order; a launch of uneven sums ends with its longest tile (in the first Gram launch of
+    // a transformer block of width 2048 some tiles' sums are four times the others', and it takes twice its work's time at full spread).
     const int idx = (int)(blockIdx.x >> 3);
     int tile = (idx / run * 8 + (int)(blockIdx.x & 7)) * run + idx % run;
     if (tile >= total) return;

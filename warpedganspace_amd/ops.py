@@ -213,11 +213,13 @@ class _LabelLogprobsFn(torch.autograd.Function):
 def label_logprobs(logits, labels, top=0, ignore_index=-100):
     """Log-probability of each row's label under softmax(logits), the entropy of the row, and its `top` most likely classes.
 
-    logits [..., V] (float32 / bfloat16 / float16, any strides; rows with adjacent scores are read in place), labels [...] int64.
+    logits [..., V] (float32 / bfloat16 / float16, any strides), labels [...] int64.  Rows with adjacent scores that are equally far apart are read in
+    place; others are copied first, a slice of positions logits[:, :-1] of [B, S, V] too (its rows have two strides).
     -> LabelLogprobs(logp [...], entropy [...], top_logp [..., top], top_index [..., top]): float32, int64 indices, equal scores in the order
     of their indices.  A label equal to ignore_index has logp 0 and passes no gradient; one that is no class otherwise gives NaN.  Rows of
     nothing but -inf: logp -inf, entropy 0, gradient 0; rows with a NaN or +inf: NaN, top_index -1.  top <= 64.
-    Differentiable in logp, entropy and top_logp (the loss and the statistics of lib/trainer.py:245-258 are made of them)."""
+    Differentiable in logp, entropy and top_logp (the loss and the statistics of lib/trainer.py:245-258 are made of them).  Both directions can be captured
+    into a graph; as with any operator of PyTorch, no eager graph of the same leaves may be alive while their backward is captured."""
     if not logits.is_cuda:
         raise L.WgsError("logits must be a GPU tensor (the HIP path has no CPU fallback)")
     if logits.dtype not in _DTYPES:

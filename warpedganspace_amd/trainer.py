@@ -199,8 +199,8 @@ class TrainStep:
         self.side_stream, self.pre_stream, main_stream = _engine_streams(device)
         # The step's critical path (shifted forward -> R -> loss -> R backward -> G backward -> Adam) runs on a stream of its own, the side work
         # that only has to be finished by the end of the step (the un-shifted pass of this / the next batch, R's weight gradients) on others.
-        # All have the default priority: work on streams of different priorities can wait for good, and a higher one for this stream was worth
-        # 0.3 % of the rate (1318.8 against 1315.0 img/s).
+        # (priority_main=False: on the caller's.)  All have the default priority: work on streams of different priorities can wait for good, and
+        # a higher one for this stream was worth 0.3 % of the rate (1318.8 against 1315.0 img/s).
         self.main_stream = main_stream if (priority_main and two_streams) else None
         self.two_streams = two_streams       # un-shifted generator pass on the side stream
         self.defer_wgrad = defer_wgrad       # R's weight gradients on the side stream, next to the generator's backward
