@@ -616,7 +616,8 @@ int wgs_label_logprobs_bwd(const void* logits, int dtype, int64_t rows, int64_t 
  * the smaller side's matrices between two products with the longer side, 1 .. 16; 0 takes 5 for bf16, 3 for fp16, 1 for fp32 and where all matrices
  * have over 128 rows and are square to a sixteenth.  Before the result's rounding, up to 3 are at most 1.4 times as far from the exact iterate as the
  * same iteration on 32-bit products (up to 1.3e-4 of its norm, at a single direction 1000 times the rest); 5 are up to 6e-4 from it, which
- * puts a bf16 result up to 11 % further away than its rounding does.
+ * puts a bf16 result up to 11 % further away than its rounding does.  Matrices of up to 16 rows or columns (the longer side up to 4096 in fp32, 1024 in 16
+ * bits) are computed in 64 bits throughout and rounded once.
  * ws: *_ws_bytes() of the same matrices, 256-byte aligned; contents do not matter before or after the call.
  */
 typedef struct wgs_matrix {

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from tests.test_orthogonalise_gpu import check
 from warpedganspace_amd import _lib as L
 from warpedganspace_amd import ops
 
@@ -33,8 +34,16 @@ def test_a_graph_that_saved_a_weight_before_the_step_is_refused(dev):
 
 
 @pytest.mark.parametrize('order', [1, -1])
-def test_a_large_matrix_beside_a_long_batch_of_small_ones(dev, order):
+def test_a_large_matrix_beside_a_long_batch_of_short_ones(dev, order):
     """Together they would pass the largest grid of the norm's launch."""
+    big, short = torch.randn(2048, 2048, device=dev), torch.randn(70000, 17, 17, device=dev)
+    got = ops.orthogonalise([big, short][::order])[::order]
+    assert torch.equal(got[0], ops.orthogonalise(big))
+    check(got[1][::997], short[::997])         # (in the launches of the large one some take another path than by themselves)
+
+
+@pytest.mark.parametrize('order', [1, -1])
+def test_a_large_matrix_beside_a_long_batch_of_single_entries(dev, order):
     big, small = torch.randn(2048, 2048, device=dev), torch.randn(70000, 1, 1, device=dev)
     got = ops.orthogonalise([big, small][::order])[::order]
     assert torch.equal(got[0], ops.orthogonalise(big))

@@ -79,11 +79,11 @@ def test_three_spans_of_which_the_outer_ones_overlap():
 def test_a_large_matrix_beside_a_long_batch_of_small_ones_is_cut_into_runs(order):
     """All matrices of a run have as many partial norms (16 bytes each) as its largest: 256 for 2048 x 2048, in at most 2^22 workgroups."""
     lib = L.lib()
-    big, small = matrix(2048, 2048, rs=2048, bs=1 << 22, obs=1 << 22), matrix(1, 1, 70000, rs=1, bs=1, obs=1)
+    big, small = matrix(2048, 2048, rs=2048, bs=1 << 22, obs=1 << 22), matrix(17, 17, 70000, rs=17, bs=289, obs=289)
 
     def need(*m):
         return lib.wgs_orthogonalise_ws_bytes(b''.join(m[::order]), len(m), 0, 5)
-    one = need(matrix(1, 1, 1, rs=1, bs=1, obs=1))
+    one = need(matrix(17, 17, 1, rs=17, bs=289, obs=289))
     assert need(small) < 70000 * (one + 64)                          # one partial norm each: a single run
     # in the large one's run at most 2^14 instances; the rest goes without it
     assert need(big, small) <= max(need(big) + (1 << 14) * (one + 64) + (16 << 22), need(small))

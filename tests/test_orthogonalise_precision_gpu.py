@@ -90,3 +90,82 @@ def test_joined_refusals(dev):
             ops.orthogonalise(x, joined=bad)
         with pytest.raises(L.WgsError, match='joined must be'):
             ops.muon_step([x], [x.clone()], [torch.zeros_like(x)], 0.1, joined=bad)
+
+
+# ---- up to 16 rows or columns: 64 bits throughout, so only the result's rounding (and 64-bit noise) separates it from the exact iterate of the
+# coefficients as the interface takes them, in fp32
+COEF32 = tuple(float(torch.tensor(c, dtype=torch.float32)) for c in ops.NS_COEFFICIENTS)
+EPS32 = float(torch.tensor(1e-7, dtype=torch.float32))
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def rounded_once(got, want, dtype, steps=5):
+    """Half a step of the type's (fp16: 2^-25 under its normal range), after one of fp32's; and the noise of 64 bits: every A_t is a polynomial of A_0, and
+    d(l (a + b l + c l^2)^2)/dl is at most a^2 < 12 on the eigenvalues, so what A_0 is off by (a few times 2^-53 of its norm) grows 12-fold a step."""
+    u = HALF[dtype] + (2.0 ** -24 if dtype != torch.float32 else 0)
+    allowed = u * (1 + 2.0 ** -8) * want.abs() + 8 * 2.0 ** -53 * 12.0 ** steps * want.abs().amax((-2, -1), keepdim=True) + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134)
+    err = (got.double() - want).abs()
+    assert (err <= allowed).all(), float((err / allowed).max())
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('shape', [(1, 1), (3, 1, 2), (1, 1000), (1000, 1), (7, 2, 3), (5, 5), (4, 40), (2, 40, 4), (16, 16), (16, 17), (15, 63), (16, 64), (2, 257, 16), (13, 1024),
+                                   (1024, 9), (3, 8, 511)], ids=str)
+def test_few_rows_are_rounded_once(dev, dtype, shape):
+    gen = torch.Generator(device=dev).manual_seed(sum(shape))
+    x = torch.randn(shape, generator=gen, device=dev).to(dtype)
+    for steps in (1, 5, 8):
+        rounded_once(ops.orthogonalise(x, steps=steps), exact(x, steps, COEF32, EPS32), dtype, steps)
+    spiked = (torch.randn(shape[:-1] + (1,), generator=gen, device=dev) * torch.randn(shape[:-2] + (1, shape[-1]), generator=gen, device=dev) + 1e-3 * x.float()).to(dtype)
+    rounded_once(ops.orthogonalise(spiked), exact(spiked, 5, COEF32, EPS32), dtype)
+    strided = torch.zeros(shape[:-1] + (shape[-1] + 3,), dtype=dtype, device=dev)[..., 2:2 + shape[-1]]
+    strided.copy_(x)
+    assert torch.equal(ops.orthogonalise(strided), ops.orthogonalise(x))
+    assert torch.equal(ops.orthogonalise([x, spiked])[1], ops.orthogonalise(spiked))
+
+
+def test_few_rows_up_to_4096_columns_in_fp32(dev):
+    gen = torch.Generator(device=dev).manual_seed(1)
+    for shape in [(4, 1025), (2, 16, 4096), (4096, 3), (1, 2500)]:
+        x = torch.randn(shape, generator=gen, device=dev)
+        rounded_once(ops.orthogonalise(x), exact(x, 5, COEF32, EPS32), torch.float32)
+
+
+def test_few_rows_with_nothing_or_no_numbers_in_them(dev):
+    gen = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randn(6, 9, 50, generator=gen, device=dev)
+    x[1] = 0
+    x[2, 3, 4] = float('nan')
+    x[3, 8, 49] = float('inf')
+    x[4, 2:] = 0
+    x[5] *= 1e-42                              # (subnormal)
+    for eps in (1e-7, 0.0):
+        o = ops.orthogonalise(x, eps=eps)
+        assert (o[1] == 0).all() and o[2].isnan().all() and o[3].isnan().all()
+        rounded_once(o[[0, 4, 5]], exact(x[[0, 4, 5]], 5, COEF32, EPS32 if eps else 0.0), torch.float32)
+    assert torch.equal(o.mT, ops.orthogonalise(x.mT.contiguous(), eps=0.0)[:]) or float((o.mT - ops.orthogonalise(x.mT.contiguous(), eps=0.0)).nan_to_num().abs().max()) < 1e-7
+    big = torch.randn(9, 50, generator=gen, device=dev) * 5e37
+    rounded_once(ops.orthogonalise(big), exact(big, 5, COEF32, EPS32), torch.float32)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('nesterov', [True, False])
+def test_steps_of_few_rows(dev, dtype, nesterov):
+    """Among larger ones in one call; momentum and update are fp32 (fused: one rounding each), the weight is rounded once."""
+    gen = torch.Generator(device=dev).manual_seed(3)
+    shapes = [(3, 7), (16, 300), (100, 20), (700, 11), (1, 1), (12, 13)]
+    R = lambda s: torch.randn(s, generator=gen, device=dev)      # noqa: E731
+    ws, gs, ms = [R(s).to(dtype) for s in shapes], [R(s).to(dtype) for s in shapes], [R(s) for s in shapes]
+    w0, m0 = [w.double() for w in ws], [m.double() for m in ms]
+    ops.muon_step(ws, gs, ms, 0.05, momentum=0.9, nesterov=nesterov, weight_decay=0.1, grad_scale=0.5, scale=1.0)
+    mu, lr, decay = (float(torch.tensor(v, dtype=torch.float32)) for v in (0.9, 0.05, 1 - 0.05 * 0.1))
+    for w, g, m, a, b in zip(ws, gs, ms, w0, m0):
+        m1 = mu * b + 0.5 * g.double()
+        assert float(((m.double() - m1).abs() - 2.0 ** -24 * m1.abs()).max()) <= 1e-30
+        if min(w.shape) > 16:
+            continue
+        u = (0.5 * g.double() + mu * m.double()) if nesterov else m.double()
+        want = decay * a - lr * exact(u.float(), 5, COEF32, EPS32)
+        # O in fp32 (2^-24 of up to 1.3), the sum of two fp32 products, the weight's type; u.float() differs by no rounding from the kernel's
+        allowed = (HALF[dtype] + 2 * 2.0 ** -24) * want.abs() + 3 * 2.0 ** -24 * (a.abs() + lr * 1.3) + (2.0 ** -25 if dtype == torch.float16 else 0)
+        assert ((w.double() - want).abs() <= allowed).all()

@@ -222,6 +222,133 @@ __global__ __launch_bounds__(512) void ortho_norm_kernel(const Group g, const Mo
     }
 }
 
+// ---- matrices of up to 16 rows (or columns): everything in 64 bits, one launch ------------------------------------------------------------------
+// The whole run is X_K = Q X_0 with Q a polynomial in A_0, and in 64 bits A_0's rounding is far under the input's own even after 16 joined steps.  (As
+// fp16 pairs, few and short sums leave a matrix of up to 8 rows up to 2.5 times as far from the exact factor as the iteration on 32-bit products: the
+// pairs' rounding, the dropped lo * lo and the matrix cores' truncation of the smaller products of a group do not average out.)  One workgroup a matrix:
+// a wave's share of A_0 from 16 columns at a time, their sum in the same order in every wave, the chain of 16 x 16 products in registers — a result's
+// layout (register v: row 4 v + lane / 16, column lane % 16) is that of either operand of the next product, all of them being symmetric —, then Q
+// times 16 columns at a time.  (As the left operand a result is its transpose: A is made symmetric in every step, else its antisymmetric rounding grows,
+// to 4e-10 in place of 6e-13 where one direction is 1000 times the rest.)  The update that is orthogonalised stays in the workspace between the two passes, in fp32, its own precision.
+// Bound by latency: of its dependent products for few columns, of one CU's loads for many.  fp32, us, the pairs' forms in brackets: 16 x 16 15 (22; 15 is
+// a host call's length), 16 x 256 15 (27), 16 x 1024 28 (45), 16 x 2048 49 (49), 16 x 4096 93 (164), 16 x 8192 180 (167); a step of one matrix 9 (27), 15 (33),
+// 44 (47), 75 (52), 144 (168), 274 (171).  So up to 4096 columns in fp32, beyond which sums are long enough for the pairs (at 4 x 1025 .. 4 x 2100 a
+// third of all matrices were over 1.5 times as far as 32-bit products, at 4 x 16000 none); in 16 bits, where joined steps take 49 at 2048 and 55 at
+// 4096 and the result's rounding hides the difference, up to 1024.
+constexpr int TINY_M = 16, TINY_N = 4096, TINY_N_16BIT = 1024, TINY_WAVES = 4;
+bool is_tiny(const Dims& d, int dtype) { return d.m <= TINY_M && d.n <= (dtype == WGS_F32 ? TINY_N : TINY_N_16BIT); }
+__host__ __device__ __forceinline__ int64_t tiny_bytes(const Dims& d) { return up((int64_t)d.m * d.n * 4, 256); }
+typedef double double4v __attribute__((ext_vector_type(4)));
+struct TinyArgs { double a, b, c; float eps; int steps; };
+template <int DT, bool STEP>
+__global__ __launch_bounds__(64 * TINY_WAVES) void ortho_tiny_kernel(const Group g, const Momentum mo, const TinyArgs ar) {
+    constexpr int U = 4;                      // groups of 16 columns in flight
+    __shared__ double part[TINY_WAVES][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4, inst = blockIdx.x;
+    const Mat& mat = g.mat[entry_of(g, inst)];
+    const Dims d = dims_of(mat.M, mat.N);
+    const int b = inst - mat.first;
+    const bool wide = mat.M <= mat.N;
+    const int64_t off = b * mat.in_bs, moff = (int64_t)b * mat.M * mat.N, ob = b * mat.out_bs;
+    float* const xs = (float*)(g.ws + mat.ws + b * tiny_bytes(d));          // [m][n]
+    auto mul = [](double x, double y, double4v z) { return __builtin_amdgcn_mfma_f64_16x16x4f64(x, y, z, 0, 0, 0); };
+    auto product = [&](const double4v& x, const double4v& y) {
+        double4v z = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) z = mul(x[s], y[s], z);
+        return z;
+    };
+    double4v A = {0.0, 0.0, 0.0, 0.0};
+    // Loads go to clamped addresses, unconditionally: they are in flight together.
+#pragma unroll 1
+    for (int k0 = 16 * U * wave; k0 < d.n; k0 += 16 * U * TINY_WAVES) {
+        float v[U][4], mm[U][4];
+        auto at = [&](int u, int t, bool& ok, int& r, int& c) {
+            const int k = k0 + 16 * u + 4 * t + q, kk = k < d.n ? k : d.n - 1, ii = i < d.m ? i : d.m - 1;
+            ok = k == kk && i == ii;
+            r = wide ? ii : kk; c = wide ? kk : ii;
+        };
+        bool ok;
+        int r, c;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                at(u, t, ok, r, c);
+                v[u][t] = load_elem<DT>(mat.in, off + (int64_t)r * mat.in_rs + c);
+                if (STEP) mm[u][t] = mat.momentum[moff + (int64_t)r * mat.N + c];
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                at(u, t, ok, r, c);
+                float x = v[u][t];
+                if (STEP) {
+                    const float gr = x * mo.grad_scale, b2 = __builtin_fmaf(mo.mu, mm[u][t], gr);
+                    if (ok) mat.momentum[moff + (int64_t)r * mat.N + c] = b2;
+                    x = mo.nesterov ? __builtin_fmaf(mo.mu, b2, gr) : b2;
+                }
+                x = ok ? x : 0.f;
+                if (ok) xs[i * d.n + k0 + 16 * u + 4 * t + q] = x;
+                A = mul((double)x, (double)x, A);
+            }
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) part[wave][v][lane] = A[v];
+    __syncthreads();                          // (the workgroup's own writes of the update, too)
+    double ss = 0.0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        A[v] = part[0][v][lane];
+#pragma unroll
+        for (int w = 1; w < TINY_WAVES; ++w) A[v] += part[w][v][lane];
+        if (4 * v + q == i) ss += A[v];
+    }
+    ss = wave_sum_d(ss);
+    // false for NaN and infinity: NaN throughout
+    const double inv = ss < 1e300 ? (ss > 0.0 ? 1.0 / (sqrt(ss) + (double)ar.eps) : 0.0) : (double)NAN;
+    A *= inv * inv;
+    double4v Q = A;
+    for (int t = 0; t < ar.steps; ++t) {
+        double4v B = product(A, A);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) B[v] = (4 * v + q == i ? ar.a : 0.0) + ar.b * A[v] + ar.c * B[v];
+        Q = t ? product(B, Q) : B;
+        if (t + 1 == ar.steps) break;
+        const double4v P = product(B, A);
+        A = 0.5 * (product(P, B) + product(B, P));       // each the other's transpose, bit for bit
+    }
+    Q *= inv;
+#pragma unroll 1
+    for (int j0 = 16 * U * wave; j0 < d.n; j0 += 16 * U * TINY_WAVES) {
+        float x[U][4], w[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int k = 4 * s + q, j = j0 + 16 * u + i, kk = k < d.m ? k : d.m - 1, jj = j < d.n ? j : d.n - 1;
+                x[u][s] = xs[kk * d.n + jj];
+                if (STEP) w[u][s] = load_elem<DT>(mat.out, ob + (int64_t)(wide ? kk : jj) * mat.out_rs + (wide ? jj : kk));
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + 16 * u + i;
+            double4v o = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) o = mul(Q[s], 4 * s + q < d.m && j < d.n ? (double)x[u][s] : 0.0, o);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int k = 4 * v + q;
+                if (k >= d.m || j >= d.n) continue;
+                float y = (float)o[v];
+                if (STEP) y = mat.decay * w[u][v] - mat.step * y;
+                store_as(DT, mat.out, ob + (int64_t)(wide ? k : j) * mat.out_rs + (wide ? j : k), y);
+            }
+        }
+    }
+}
+
 // ---- 2. scalars and the planes of X and X^T -----------------------------------------------------------------------------------------
 struct Bounds { float eps; int steps; float grow[MAX_STEPS + 1], cap[MAX_STEPS + 1]; };      // |A_t| <= min(D0 grow[t], cap[t])
 __device__ __forceinline__ float pow2_under(float bound, int top, int lo, int hi) {        // 2^(top - ceil(log2 bound)), clamped
@@ -1335,7 +1462,8 @@ struct Plan { int phases, len[MAX_STEPS]; int planes, npx, nt, ns; };
 //   ... of 0.001, 0.0001                 4e-4      1.3e-4    1.3e-4    6e-4
 //   eight directions in noise of 0.01    6e-5      4e-5      3e-5      2e-4
 //   a third of the rank; 5 decades       9e-6      1.3e-5    8e-6      3e-4
-// Single iterations are at most 1.4 times as far as 32-bit products (mostly nearer: the sums have fewer roundings), (3, 2) as good as they.
+// Single iterations are at most 1.4 times as far as 32-bit products (mostly nearer: the sums have fewer roundings), (3, 2) as good as they.  (A single
+// matrix of 17 .. 24 rows can be up to 2.5 times as far: two draws of a few roundings.  Up to 16 rows go through ortho_tiny_kernel.)
 // Five are not: they put a bf16 result up to 11 % further from the exact factor than its rounding does, and save 1.4 ms of 6.1 at 4096 x 16384
 // (single iterations: 10.3), 30 us of 136 at 64 of 128 x 512.  So bf16 takes five, fp16 three, fp32 one, where the caller names no number;
 // nearly square matrices of over 128 rows, whose products with X cost no more than those they replace, one whatever the type (bf16 singles / (3, 2) /
@@ -1348,7 +1476,7 @@ Plan plan_of(int dtype, bool step, int steps, const wgs_matrix* mats, int count)
         if (dtype != WGS_F32)
             for (int i = 0; i < count; ++i) {
                 const Dims d = dims_of(mats[i].rows, mats[i].cols);
-                if (mats[i].batch && (d.m <= 128 || d.n - d.m > d.m / 16)) most = dtype == WGS_BF16 ? 5 : 3;
+                if (mats[i].batch && !is_tiny(d, dtype) && (d.m <= 128 || d.n - d.m > d.m / 16)) most = dtype == WGS_BF16 ? 5 : 3;
             }
     }
     p.phases = (steps + most - 1) / most;
@@ -1374,23 +1502,26 @@ int norm_blocks(int64_t elements) {               // 64 elements a thread where 
     return sb < 1 ? 1 : (sb > STAT_BLOCKS ? STAT_BLOCKS : (int)sb);
 }
 
-// The matrices in runs of at most MAX_MATS entries, NORM_BLOCKS and CHUNK_BYTES (or one matrix); batches are cut where they have to be.
+constexpr int64_t TINY_BLOCKS = 1 << 22;         // (the same for the matrices of up to 16 rows, a workgroup of 256 each)
+
+// The matrices, those of up to 16 rows or the others, in runs of at most MAX_MATS entries, NORM_BLOCKS (TINY_BLOCKS) and CHUNK_BYTES (or one matrix);
+// batches are cut where they have to be.
 struct Cursor { int entry = 0, done = 0; };
-int64_t next_chunk(const wgs_matrix* mats, int count, const Plan& p, Cursor& c, Group& g) {
+int64_t next_chunk(const wgs_matrix* mats, int count, const Plan& p, bool tiny, Cursor& c, Group& g) {
     int64_t bytes = 0;
     g.count = 0; g.instances = 0;
     int64_t most = 0;
     while (c.entry < count && g.count < MAX_MATS) {
         const wgs_matrix& w = mats[c.entry];
         const int left = w.batch - c.done;
-        if (left <= 0) { ++c.entry; c.done = 0; continue; }
         const Dims d = dims_of(w.rows, w.cols);
-        int64_t one = instance_bytes(d, p.npx, p.nt, p.ns);
-        if (is_small(d) && small_bytes(d) > one) one = small_bytes(d);
+        if (left <= 0 || is_tiny(d, g.dtype) != tiny) { ++c.entry; c.done = 0; continue; }
+        int64_t one = tiny ? tiny_bytes(d) : instance_bytes(d, p.npx, p.nt, p.ns);
+        if (!tiny && is_small(d) && small_bytes(d) > one) one = small_bytes(d);
         const int64_t elements = (int64_t)w.rows * w.cols, largest = elements > most ? elements : most;
         int64_t fit = (CHUNK_BYTES - bytes) / one;
         if (fit < 1 && !g.count) fit = 1;
-        const int64_t room = NORM_BLOCKS / norm_blocks(largest) - g.instances;
+        const int64_t room = (tiny ? TINY_BLOCKS : NORM_BLOCKS / norm_blocks(largest)) - g.instances;
         if (fit > room) fit = room;
         if (fit < 1) break;
         const int take = fit < left ? (int)fit : left;
@@ -1412,6 +1543,7 @@ int64_t next_chunk(const wgs_matrix* mats, int count, const Plan& p, Cursor& c, 
         if (take < left) break;
     }
     if (!g.count) return 0;
+    if (tiny) return bytes;
     g.stat_blocks = norm_blocks(most);
     g.info = up((int64_t)g.instances * g.stat_blocks * (int64_t)sizeof(Part), 256);
     int64_t head = g.info + up((int64_t)g.instances * INFO * 4, 256);
@@ -1444,15 +1576,15 @@ const char* check_mats(const wgs_matrix* mats, int count, int dtype, bool step, 
 
 int64_t workspace(const wgs_matrix* mats, int count, int dtype, bool step, int steps) {
     const Plan p = plan_of(dtype, step, steps, mats, count);
-    Cursor c;
     Group g;
     g.dtype = dtype;
     int64_t need = 0;
-    for (;;) {
-        const int64_t b = next_chunk(mats, count, p, c, g);
-        if (!b) return need;
-        if (b > need) need = b;
+    for (bool tiny : {true, false}) {
+        Cursor c;
+        while (const int64_t b = next_chunk(mats, count, p, tiny, c, g))
+            if (b > need) need = b;
     }
+    return need;
 }
 
 // the largest |a + b l + c l^2| on [0, top], and of l (a + b l + c l^2)^2
@@ -1585,6 +1717,13 @@ void launch_small(const Group& g, const Momentum& mo, SmallArgs ar, hipStream_t 
     }
 }
 
+template <int DT>
+void launch_tiny(const Group& g, const Momentum& mo, const TinyArgs& ar, hipStream_t st) {
+    const dim3 gr((unsigned)g.instances), bl(64 * TINY_WAVES);
+    if (g.step) WGS_LAUNCH((ortho_tiny_kernel<DT, true>), gr, bl, 0, st, g, mo, ar);
+    else WGS_LAUNCH((ortho_tiny_kernel<DT, false>), gr, bl, 0, st, g, mo, ar);
+}
+
 int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step, const Momentum& mo, int steps, double a, double b, double c, float eps, void* ws,
         int64_t ws_bytes, hipStream_t st) {
     const char* bad = check_mats(mats, count, dtype, step, steps);
@@ -1606,13 +1745,19 @@ int run(const char* who, const wgs_matrix* mats, int count, int dtype, bool step
         grow = fmin(grow * q[t] * q[t], 1e30); cap = next;
     }
     const Plan p = plan_of(dtype, step, steps, mats, count);
-    Cursor cur;
+    Cursor cur, tiny;
     Group g;
     g.dtype = dtype; g.step = step; g.npx = p.npx; g.nt = p.nt; g.ns = p.ns; g.ws = (unsigned char*)ws;
     SmallArgs sm;
     sm.bd = bd; sm.a = (float)a; sm.b = (float)b; sm.c = (float)c;
     for (int t = 0; t < steps; ++t) sm.sb[t] = (float)ldexp(1.0, 14 - ceil_log2(q[t]));
-    while (next_chunk(mats, count, p, cur, g) > 0) {
+    while (next_chunk(mats, count, p, true, tiny, g) > 0) {
+        const TinyArgs ta = {a, b, c, eps, steps};
+        if (dtype == WGS_F32) launch_tiny<WGS_F32>(g, mo, ta, st);
+        else if (dtype == WGS_BF16) launch_tiny<WGS_BF16>(g, mo, ta, st);
+        else launch_tiny<WGS_F16>(g, mo, ta, st);
+    }
+    while (next_chunk(mats, count, p, false, cur, g) > 0) {
         if (all_small(g, p, steps)) {
             launch_small(g, mo, sm, st);
             continue;

@@ -300,7 +300,8 @@ def orthogonalise(x, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7, joined=Non
     joined: the most iterations that run on the smaller side's matrices alone between two products with the longer side.  None takes 5 for bfloat16,
     3 for float16, 1 for float32 and for matrices (all those of a call) of over 128 rows that are square to a sixteenth.  Up to 3 come as close to the
     exact iterate as 32-bit products do (within 1.4 times their distance); 5 are faster on wide matrices and put a bfloat16 result up to 11 % further from
-    it than its rounding does, where one direction outweighs the rest."""
+    it than its rounding does, where one direction outweighs the rest.  Matrices whose smaller side is at most 16 (and the longer one at most 4096 in float32,
+    1024 in 16 bits) are computed in 64 bits and rounded once."""
     many = isinstance(x, (list, tuple))
     xs = list(x) if many else [x]
     joined = _joined(joined)
