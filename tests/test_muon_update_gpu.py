@@ -78,3 +78,34 @@ def test_a_gradient_that_was_made_anew_is_not_taken_for_the_old_one(dev):
     plan = ops.MuonUpdate([w], [g], [m])
     w.grad = None
     plan.step(0.1)
+
+
+def test_captured_steps_of_few_rows_among_others(dev):
+    """Replays read the buffers' current contents, with eager work in between; two graphs do not share a workspace."""
+    shapes = [(5, 70), (40, 90), (900, 16), (1, 1)]
+
+    def state(seed):
+        gen = torch.Generator(device=dev).manual_seed(seed)
+        return [[torch.randn(s, generator=gen, device=dev) for s in shapes] for _ in range(3)]
+    cap, ref = [state(1), state(2)], [state(1), state(2)]
+    ops.muon_step(*state(3), 0.1)
+    torch.cuda.synchronize()
+    graphs = []
+    for s in cap:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.muon_step(*s, 0.1, weight_decay=0.1)
+        graphs.append(g)
+    for k in range(3):
+        fresh = state(10 + k)[1]
+        for i in (0, 1):
+            for a, b, new in zip(cap[i][1], ref[i][1], fresh):
+                a.copy_(new * (i + 1))
+                b.copy_(new * (i + 1))
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            ops.muon_step(*ref[i], 0.1, weight_decay=0.1)
+            for a, b in zip(cap[i][0] + cap[i][2], ref[i][0] + ref[i][2]):
+                assert torch.equal(a, b), (k, i)
